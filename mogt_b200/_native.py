@@ -22,7 +22,25 @@ OK, ERR_SHAPE, ERR_DTYPE, ERR_ALIGN, ERR_LAUNCH, ERR_TIMEOUT, ERR_WORKSPACE, ERR
 
 _vp, _i64, _int, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_size_t
 
-# name -> (restype, argtypes); must match include/mogt_scan.h
+_f32 = ctypes.c_float
+
+
+class SelectiveArgs(ctypes.Structure):
+    """mogt_selective_args of include/mogt_selective.h."""
+    _fields_ = ([(n, _vp) for n in ("u", "delta", "z", "Bm", "Cm")]
+                + [(n, _i64) for n in ("u_sb", "u_sl", "delta_sb", "delta_sl", "z_sb", "z_sl",
+                                       "B_sb", "B_sl", "B_sg", "C_sb", "C_sl", "C_sg")]
+                + [(n, _vp) for n in ("A", "Dskip", "bias", "init", "lengths")]
+                + [(n, _i64) for n in ("B", "L", "D", "N", "G")]
+                + [("softplus", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+                + [(n, _vp) for n in ("out", "final_state", "saved", "dout")]
+                + [("dout_sb", _i64), ("dout_sl", _i64)]
+                + [(n, _vp) for n in ("dfinal", "du", "ddelta", "dz", "dB", "dC", "dA", "dD", "dbias",
+                                      "dinit", "scratch")]
+                + [("scratch_bytes", _sz)])
+
+
+# name -> (restype, argtypes); must match include/*.h
 SIGNATURES = {
     "mogt_abi_version": (_int, []),
     "mogt_status_string": (ctypes.c_char_p, [_int]),
@@ -53,6 +71,26 @@ SIGNATURES = {
     "mogt_affine_scan_workspace_bytes": (_sz, [_i64] * 4),
     "mogt_affine_scan_fwd": (_int, [_vp] * 4 + [_i64] * 4 + [_int] * 4 + [_vp, _sz, _vp]),
     "mogt_affine_grad_u": (_int, [_vp] * 3 + [_i64] * 4 + [_int, _vp]),
+    "mogt_causal_conv_fwd": (_int, [_vp, _i64, _i64] + [_vp] * 6 + [_i64] * 4 + [_int] * 3 + [_vp]),
+    "mogt_causal_conv_bwd_scratch_bytes": (_sz, [_i64] * 4),
+    "mogt_causal_conv_bwd": (_int, [_vp, _i64, _i64] + [_vp] * 5 + [_i64, _i64] + [_vp] * 5 + [_i64] * 4
+                             + [_int] * 3 + [_vp, _sz, _vp]),
+    "mogt_causal_conv_step": (_int, [_vp, _i64] + [_vp] * 5 + [_i64] * 3 + [_int] * 3 + [_vp]),
+    "mogt_selective_saved_bytes": (_sz, [_i64] * 4),
+    "mogt_selective_fwd_scratch_bytes": (_sz, [_i64] * 5),
+    "mogt_selective_bwd_scratch_bytes": (_sz, [_i64] * 5),
+    "mogt_selective_scan_fwd": (_int, [ctypes.POINTER(SelectiveArgs), _vp]),
+    "mogt_selective_scan_bwd": (_int, [ctypes.POINTER(SelectiveArgs), _vp]),
+    "mogt_selective_step": (_int, [_vp, _vp] + [_vp, _i64] * 3 + [_vp, _i64, _i64] * 2 + [_vp] * 4 + [_i64] * 4
+                            + [_int, _int, _vp]),
+    "mogt_logprob_fwd": (_int, [_vp, _i64, _i64, _vp, _vp] + [_i64] * 3 + [_int] + [_vp] * 3),
+    "mogt_logprob_bwd": (_int, [_vp, _i64, _i64] + [_vp] * 4 + [_i64, _vp, _vp, _i64, _i64] + [_i64] * 3
+                         + [_int, _vp]),
+    "mogt_policy_loss_scratch_bytes": (_sz, [_i64] * 2),
+    "mogt_policy_loss": (_int, [_vp, _i64, _i64] + [_vp] * 5 + [_i64, _i64] + [_f32] * 3 + [_vp] * 5
+                         + [_i64, _i64] + [_i64] * 3 + [_int, _vp, _sz, _vp]),
+    "mogt_preference_pairs": (_int, [_vp, _vp, _i64, _i64, _f32, _f32] + [_vp] * 4),
+    "mogt_scale_unless_one": (_int, [_vp, _i64, _int, _vp, _vp]),
 }
 
 _lib = None

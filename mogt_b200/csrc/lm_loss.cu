@@ -1,0 +1,395 @@
+// Post-training losses on logits rows: label log-probabilities, the clipped
+// policy loss with a KL term, the paired preference loss, and their gradients.
+//   lp = x_l - lse,  lse = m + log sum_v exp(x_v - m);
+//   d lp / d x_v = [v = l] - exp(x_v - lse).
+// One multiply-add, one exponential and a compare or two per logit of 2 or 4
+// bytes: HBM bounds all of it.  A CTA takes a row; the maximum and the sum of
+// exponentials are carried together over one pass (rescaled when the maximum
+// grows).  The policy loss knows a token's coefficient as soon as the row's
+// sum is known, so its gradient row is written by the same CTA at once, while
+// the row it has just read is still in L2: one read and one write of the
+// logits in HBM for the loss and its gradient.
+#include <type_traits>
+
+#include "../../include/mogt_lm_loss.h"
+#include "selective.cuh"
+
+namespace mogt {
+namespace lml {
+
+constexpr int NT = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Rows {
+  const void* logits;
+  int64_t sb, sl;
+  const int64_t* labels;
+  const uint8_t* mask;
+  int64_t L, V, rows;
+  void* d;
+  int64_t d_sb, d_sl;
+  float* lp;
+  float2* stats;
+};
+
+struct Policy {
+  const float *old, *ref, *adv;
+  int64_t adv_sb, adv_sl;
+  float lo, hi, kl;
+  const float* inv_n;
+  float *tok, *coef;
+};
+
+__device__ __forceinline__ bool counts(const Rows& r, int64_t row) {
+  return (!r.mask || r.mask[row]) && r.labels[row] >= 0;
+}
+
+// exp(x - m) with the subtraction first: exact for equal values of any size
+// (rows of the type's lowest value included).
+__device__ __forceinline__ float exp_diff(float x, float m) { return fast_exp2((x - m) * kLog2e); }
+
+struct MS {
+  float m, s;
+};
+__device__ __forceinline__ MS merge(MS a, MS b) {
+  const float m = fmaxf(a.m, b.m);
+  MS r{m, 0.f};
+  // an empty side (s = 0, m = -inf) adds nothing; a NaN sum is kept
+  if (a.s != 0.f) r.s += a.s * exp_diff(a.m, m);
+  if (b.s != 0.f) r.s += b.s * exp_diff(b.m, m);
+  return r;
+}
+__device__ __forceinline__ MS one(float x) { return MS{x, x == -INFINITY ? 0.f : 1.f}; }
+
+// A row as a head of single elements up to a 16-byte boundary, whole 16-byte
+// vectors, and a tail.
+template <typename T>
+struct Split {
+  static constexpr int VEC = 16 / (int)sizeof(T);
+  int64_t head, nvec, tail0;
+  __device__ Split(const T* x, int64_t V) {
+    const int64_t mis = (reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T);
+    head = mis ? VEC - mis : 0;
+    if (head > V) head = V;
+    nvec = (V - head) / VEC;
+    tail0 = head + nvec * VEC;
+  }
+};
+
+// Maximum and sum of exponentials of a row, known to every thread.
+template <typename T>
+__device__ MS row_stats(const T* x, int64_t V, MS* red) {
+  constexpr int VEC = Split<T>::VEC;
+  const Split<T> sp(x, V);
+  float m = -INFINITY, s = 0.f;
+  const T* xv = x + sp.head;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < sp.nvec; i += NT) {
+    Pack<T, VEC> v;
+    v.load(xv + i * VEC);
+    float f[VEC], mx = v.f(0);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      f[k] = v.f(k);
+      mx = fmaxf(mx, f[k]);
+    }
+    const float mn = fmaxf(m, mx);
+    const float ref = mn == -INFINITY ? 0.f : mn;
+    s *= exp_diff(m, ref);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) s += exp_diff(f[k], ref);
+    m = mn;
+  }
+  MS a{m, s};
+  const int64_t edge = threadIdx.x;
+  if (edge < sp.head) a = merge(a, one(to_f32(x[edge])));
+  if (sp.tail0 + edge < V) a = merge(a, one(to_f32(x[sp.tail0 + edge])));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    a = merge(a, MS{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  __syncthreads();
+  if (lane == 0) red[w] = a;
+  __syncthreads();
+  a = red[lane % (NT / 32)];
+#pragma unroll
+  for (int o = NT / 64; o > 0; o >>= 1)
+    a = merge(a, MS{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o)});
+  return a;
+}
+
+// d[v] = c * ([v = label] - p_v), p_v = exp(x_v - m) / s.
+template <typename T>
+__device__ void write_grad(const T* x, T* d, int64_t V, int64_t label, float c, float m, float inv_s) {
+  constexpr int VEC = Split<T>::VEC;
+  const Split<T> sp(x, V);
+  const float f = -c * inv_s;
+  const T* xv = x + sp.head;
+  T* dv = d + sp.head;
+  if (((reinterpret_cast<uintptr_t>(dv)) & 15u) == 0) {
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < sp.nvec; i += NT) {
+      Pack<T, VEC> v, o;
+      v.load(xv + i * VEC);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) o.set(k, f * exp_diff(v.f(k), m));
+      o.store(dv + i * VEC);
+    }
+  } else {
+    for (int64_t i = threadIdx.x; i < sp.nvec * VEC; i += NT) dv[i] = from_f32<T>(f * exp_diff(to_f32(xv[i]), m));
+  }
+  const int64_t edge = threadIdx.x;
+  if (edge < sp.head) d[edge] = from_f32<T>(f * exp_diff(to_f32(x[edge]), m));
+  if (sp.tail0 + edge < V) d[sp.tail0 + edge] = from_f32<T>(f * exp_diff(to_f32(x[sp.tail0 + edge]), m));
+  __syncthreads();
+  if (threadIdx.x == 0 && label < V) d[label] = from_f32<T>(fmaf(f, exp_diff(to_f32(x[label]), m), c));
+}
+
+template <typename T>
+__device__ void write_zero(T* d, int64_t V) {
+  constexpr int VEC = Split<T>::VEC;
+  const Split<T> sp(d, V);
+  Pack<T, VEC> z;
+  z.zero();
+  for (int64_t i = threadIdx.x; i < sp.nvec; i += NT) z.store(d + sp.head + i * VEC);
+  const int64_t edge = threadIdx.x;
+  if (edge < sp.head) d[edge] = from_f32<T>(0.f);
+  if (sp.tail0 + edge < V) d[sp.tail0 + edge] = from_f32<T>(0.f);
+}
+
+__device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); }
+
+// One CTA per row: log-probability; with POLICY the token's loss and
+// coefficient, and with GRAD the row of the gradient.
+template <typename T, bool POLICY, bool GRAD>
+__global__ void __launch_bounds__(NT) rows_kernel(const Rows r, const Policy q) {
+  __shared__ MS red[NT / 32];
+  const int64_t row = blockIdx.x, b = row / r.L, l = row % r.L;
+  T* d = GRAD ? static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl : nullptr;
+  if (!counts(r, row)) {
+    if (GRAD) write_zero(d, r.V);
+    if (threadIdx.x == 0) {
+      r.lp[row] = 0.f;
+      if (r.stats) r.stats[row] = make_float2(0.f, 1.f);
+      if (POLICY) q.tok[row] = q.coef[row] = 0.f;
+    }
+    return;
+  }
+  const T* x = static_cast<const T*>(r.logits) + b * r.sb + l * r.sl;
+  const int64_t label = r.labels[row];
+  const MS a = row_stats(x, r.V, red);
+  const float lp = label < r.V ? (to_f32(x[label]) - a.m) - logf(a.s) : nan_f32();
+  float tok = 0.f, c = 0.f;
+  if (POLICY) {
+    const float adv = q.adv[b * q.adv_sb + l * q.adv_sl];
+    const float rr = expf(lp - q.old[row]);
+    const float s1 = rr * adv, s2 = fminf(fmaxf(rr, q.lo), q.hi) * adv;
+    tok = -fminf(s1, s2);
+    c = s1 <= s2 ? -s1 : 0.f;
+    if (s1 != s1) tok = c = s1;  // NaN is not dropped by the minimum
+    if (q.ref) {
+      const float dd = q.ref[row] - lp, e = expm1f(dd);
+      tok = fmaf(q.kl, e - dd, tok);
+      c = fmaf(-q.kl, e, c);
+    }
+    c *= *q.inv_n;
+  }
+  if (threadIdx.x == 0) {
+    r.lp[row] = lp;
+    if (r.stats) r.stats[row] = make_float2(a.m, a.s);
+    if (POLICY) {
+      q.tok[row] = tok;
+      q.coef[row] = c;
+    }
+  }
+  if (GRAD) write_grad(x, d, r.V, label, c, a.m, 1.f / a.s);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(NT) rows_bwd_kernel(const Rows r, const float* coef, int64_t coef_div,
+                                                      const float* scale) {
+  const int64_t row = blockIdx.x, b = row / r.L, l = row % r.L;
+  T* d = static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl;
+  if (!counts(r, row)) {
+    write_zero(d, r.V);
+    return;
+  }
+  float c = coef[row / coef_div];
+  if (scale) c *= *scale;
+  const int64_t label = r.labels[row];
+  if (label >= r.V) c = nan_f32();
+  const float2 st = r.stats[row];
+  write_grad(static_cast<const T*>(r.logits) + b * r.sb + l * r.sl, d, r.V, label, c, st.x, 1.f / st.y);
+}
+
+// 1 / max(number of counting tokens, 1).
+__global__ void __launch_bounds__(1024) count_kernel(const Rows r, float* inv_n) {
+  __shared__ int64_t sm[32];
+  int64_t n = 0;
+  for (int64_t i = threadIdx.x; i < r.rows; i += 1024) n += counts(r, i);
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    n = 0;
+    for (int i = 0; i < 32; ++i) n += sm[i];
+    *inv_n = 1.f / (float)(n > 0 ? n : 1);
+  }
+}
+
+__device__ double block_sum_1024(double v, double* sm) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < 32; ++i) v += sm[i];
+  return v;
+}
+
+__global__ void __launch_bounds__(1024) token_mean_kernel(const float* tok, int64_t rows, const float* inv_n,
+                                                          float* loss) {
+  __shared__ double sm[32];
+  double v = 0.0;
+  for (int64_t i = threadIdx.x; i < rows; i += 1024) v += tok[i];
+  v = block_sum_1024(v, sm);
+  if (threadIdx.x == 0) *loss = (float)(v * (double)*inv_n);
+}
+
+__device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
+
+// One CTA: a warp sums a sequence's log-probabilities, a thread takes a pair.
+__global__ void __launch_bounds__(1024) pairs_kernel(const float* lp, const float* ref, int64_t P, int64_t L,
+                                                     float beta, float eps, float* loss, float* seq, float* coef) {
+  __shared__ double sm[32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int64_t i = w; i < 2 * P; i += 32) {
+    double v = 0.0;
+    for (int64_t l = lane; l < L; l += 32) v += lp[i * L + l];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) seq[i] = (float)v;
+  }
+  __syncthreads();
+  double tot = 0.0;
+  for (int64_t i = threadIdx.x; i < P; i += 1024) {
+    const float x = beta * ((seq[i] - ref[i]) - (seq[P + i] - ref[P + i]));
+    tot -= (1.f - eps) * log_sigmoid(x) + eps * log_sigmoid(-x);
+    const float c = beta / (float)P * (eps / (1.f + expf(-x)) - (1.f - eps) / (1.f + expf(x)));
+    coef[i] = c;
+    coef[P + i] = -c;
+  }
+  tot = block_sum_1024(tot, sm);
+  if (threadIdx.x == 0) *loss = (float)(tot / (double)(P > 0 ? P : 1));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) scale_kernel(T* x, int64_t n, const float* scale) {
+  const float s = *scale;
+  if (s == 1.f) return;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    x[i] = from_f32<T>(s * to_f32(x[i]));
+}
+
+template <typename F>
+int by_type(int dtype, F&& f) {
+  switch (dtype) {
+    case MOGT_DTYPE_F32: return f(float{});
+    case MOGT_DTYPE_BF16: return f(__nv_bfloat16{});
+    case MOGT_DTYPE_F16: return f(__half{});
+    default: return MOGT_ERR_DTYPE;
+  }
+}
+
+inline int check(int64_t B, int64_t L, int64_t V, int dtype) {
+  if (B < 0 || L < 0 || V <= 0) return MOGT_ERR_SHAPE;
+  if (dtype < 0 || dtype > 2) return MOGT_ERR_DTYPE;
+  if (B * L >= ((int64_t)1 << 31)) return MOGT_ERR_UNSUPPORTED;
+  return MOGT_OK;
+}
+
+}  // namespace lml
+}  // namespace mogt
+
+using namespace mogt;
+using namespace mogt::lml;
+
+extern "C" int mogt_logprob_fwd(const void* logits, int64_t sb, int64_t sl, const int64_t* labels,
+                                const uint8_t* mask, int64_t B, int64_t L, int64_t V, int dtype, float* logprobs,
+                                float* stats, void* stream) {
+  if (int st = check(B, L, V, dtype)) return st;
+  if (B * L == 0) return MOGT_OK;
+  if (!logits || !labels || !logprobs) return MOGT_ERR_ARG;
+  Rows r{logits, sb, sl, labels, mask, L, V, B * L, nullptr, 0, 0, logprobs, reinterpret_cast<float2*>(stats)};
+  return by_type(dtype, [&](auto t) {
+    rows_kernel<decltype(t), false, false><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, Policy{});
+    return mogt_host::launch_status();
+  });
+}
+
+extern "C" int mogt_logprob_bwd(const void* logits, int64_t sb, int64_t sl, const int64_t* labels,
+                                const uint8_t* mask, const float* stats, const float* coef, int64_t coef_div,
+                                const float* scale, void* dlogits, int64_t d_sb, int64_t d_sl, int64_t B, int64_t L,
+                                int64_t V, int dtype, void* stream) {
+  if (int st = check(B, L, V, dtype)) return st;
+  if (coef_div <= 0) return MOGT_ERR_SHAPE;
+  if (B * L == 0) return MOGT_OK;
+  if (!logits || !labels || !stats || !coef || !dlogits) return MOGT_ERR_ARG;
+  Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, nullptr,
+         const_cast<float2*>(reinterpret_cast<const float2*>(stats))};
+  return by_type(dtype, [&](auto t) {
+    rows_bwd_kernel<decltype(t)><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, coef, coef_div, scale);
+    return mogt_host::launch_status();
+  });
+}
+
+extern "C" size_t mogt_policy_loss_scratch_bytes(int64_t B, int64_t L) {
+  return B < 0 || L < 0 ? 0 : (size_t)(B * L + 1) * sizeof(float);
+}
+
+extern "C" int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, const int64_t* labels,
+                                const uint8_t* mask, const float* old_logprobs, const float* ref_logprobs,
+                                const float* adv, int64_t adv_sb, int64_t adv_sl, float clip_low, float clip_high,
+                                float kl_coef, float* loss, float* logprobs, float* stats, float* coef, void* dlogits,
+                                int64_t d_sb, int64_t d_sl, int64_t B, int64_t L, int64_t V, int dtype,
+                                void* scratch, size_t scratch_bytes, void* stream) {
+  if (int st = check(B, L, V, dtype)) return st;
+  if (!loss) return MOGT_ERR_ARG;
+  if (B * L > 0 && (!logits || !labels || !old_logprobs || !adv || !logprobs || !coef)) return MOGT_ERR_ARG;
+  if (!scratch || scratch_bytes < mogt_policy_loss_scratch_bytes(B, L)) return MOGT_ERR_WORKSPACE;
+  float* inv_n = static_cast<float*>(scratch);
+  Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, logprobs, reinterpret_cast<float2*>(stats)};
+  Policy q{old_logprobs, ref_logprobs, adv, adv_sb, adv_sl, 1.f - clip_low, 1.f + clip_high, kl_coef, inv_n,
+           inv_n + 1, coef};
+  cudaStream_t s = (cudaStream_t)stream;
+  return by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    count_kernel<<<1, 1024, 0, s>>>(r, inv_n);
+    if (r.rows > 0) {
+      if (dlogits) rows_kernel<T, true, true><<<(unsigned)r.rows, NT, 0, s>>>(r, q);
+      else rows_kernel<T, true, false><<<(unsigned)r.rows, NT, 0, s>>>(r, q);
+    }
+    token_mean_kernel<<<1, 1024, 0, s>>>(q.tok, r.rows, inv_n, loss);
+    return mogt_host::launch_status();
+  });
+}
+
+extern "C" int mogt_preference_pairs(const float* logprobs, const float* ref, int64_t P, int64_t L, float beta,
+                                     float eps, float* loss, float* seq, float* coef, void* stream) {
+  if (P < 0 || L < 0) return MOGT_ERR_SHAPE;
+  if (!loss || (P > 0 && (!ref || !seq || !coef || (L > 0 && !logprobs)))) return MOGT_ERR_ARG;
+  pairs_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(logprobs, ref, P, L, beta, eps, loss, seq, coef);
+  return mogt_host::launch_status();
+}
+
+extern "C" int mogt_scale_unless_one(void* x, int64_t n, int dtype, const float* scale, void* stream) {
+  if (n < 0) return MOGT_ERR_SHAPE;
+  if (n == 0) return MOGT_OK;
+  if (!x || !scale) return MOGT_ERR_ARG;
+  const int64_t blocks = (n + 1023) / 1024;
+  return by_type(dtype, [&](auto t) {
+    using T = decltype(t);
+    scale_kernel<T><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, (cudaStream_t)stream>>>(
+        static_cast<T*>(x), n, scale);
+    return mogt_host::launch_status();
+  });
+}

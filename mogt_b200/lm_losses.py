@@ -1,0 +1,250 @@
+"""Losses of post-training on logits: the log-probabilities of labels, the
+clipped policy loss with a KL term, and the paired preference loss.
+
+Next to ``chunked_lm_loss`` (plain cross-entropy from hidden states) these
+take logits [B, L, V] in bfloat16, float16 or float32 as a head produces them
+(rows of a wider, padded head are fine as a view) and labels [B, L] aligned
+with them: ``labels[b, l]`` is scored by ``logits[b, l]``.
+
+A token counts when ``mask`` (bool, default: all) is set and its label is not
+negative (-100 by convention).  Rows that do not count are not read, whatever
+they hold; their log-probability, loss and gradient are zero, and a batch
+without any counting token has loss 0.  A counting label >= V gives NaN (it
+is not checked on the host, which would have to wait for the device).
+
+Statistics are fp32, sums over tokens and pairs fp64 in a fixed order, so
+results do not vary between runs.  Only the logits receive a gradient.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _native as N
+from .selective import _DTYPES, _cuda, _ptr, _stream
+
+__all__ = ["token_logprobs", "policy_loss", "preference_loss"]
+
+
+def _rows(what, logits, labels, mask):
+    if logits.ndim != 3 or logits.dtype not in _DTYPES:
+        raise ValueError(f"{what}: logits must be [B, L, V] bfloat16, float16 or float32")
+    if logits.shape[2] < 1:
+        raise ValueError(f"{what}: the vocabulary is empty")
+    if labels.shape != logits.shape[:2] or labels.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what}: labels must be [B, L] int64 or int32")
+    if mask is not None and (mask.shape != labels.shape or mask.dtype != torch.bool):
+        raise ValueError(f"{what}: mask must be [B, L] bool")
+    if logits.stride(2) != 1 and logits.shape[2] > 1:
+        logits = logits.contiguous()
+    return logits, labels.to(torch.int64).contiguous(), None if mask is None else mask.contiguous()
+
+
+def _grad_like(logits):
+    """An empty [B, L, V] whose rows start at the same offsets from a 16-byte
+    boundary as those of logits, so that both are accessed 16 bytes at a time."""
+    B, L, V = logits.shape
+    sb, sl, _ = logits.stride()
+    if sl >= V and sb == L * sl and logits.data_ptr() % 16 == 0:
+        return torch.empty(B, L, sl, dtype=logits.dtype, device=logits.device)[..., :V]
+    return torch.empty(B, L, V, dtype=logits.dtype, device=logits.device)
+
+
+def _logprob_fwd(logits, labels, mask, want_stats):
+    B, L, V = logits.shape
+    dev = logits.device
+    lp = torch.empty(B, L, dtype=torch.float32, device=dev)
+    stats = torch.empty(B, L, 2, dtype=torch.float32, device=dev) if want_stats else None
+    with torch.cuda.device(dev):
+        N.check(N.lib().mogt_logprob_fwd(logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
+                                         _ptr(mask), B, L, V, N.dtype_code(logits.dtype), lp.data_ptr(), _ptr(stats),
+                                         _stream(dev)), "mogt_logprob_fwd")
+    return lp, stats
+
+
+def _logprob_bwd(logits, labels, mask, stats, coef, coef_div, scale):
+    B, L, V = logits.shape
+    dev = logits.device
+    d = _grad_like(logits)
+    scale = None if scale is None else scale.to(torch.float32).contiguous()
+    with torch.cuda.device(dev):
+        N.check(N.lib().mogt_logprob_bwd(logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
+                                         _ptr(mask), stats.data_ptr(), coef.data_ptr(), coef_div, _ptr(scale),
+                                         d.data_ptr(), d.stride(0), d.stride(1), B, L, V, N.dtype_code(logits.dtype),
+                                         _stream(dev)), "mogt_logprob_bwd")
+    return d
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, mask):
+        lp, stats = _logprob_fwd(logits, labels, mask, True)
+        ctx.save_for_backward(logits, labels, mask, stats)
+        return lp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        logits, labels, mask, stats = ctx.saved_tensors
+        return _logprob_bwd(logits, labels, mask, stats, g.to(torch.float32).contiguous(), 1, None), None, None
+
+
+def token_logprobs(logits, labels, *, mask=None):
+    """log softmax(logits)[label] per token, fp32 [B, L]; 0 where a token does
+    not count.  Differentiable in logits."""
+    what = "token_logprobs"
+    _cuda(what, logits, labels, mask)
+    logits, labels, mask = _rows(what, logits, labels, mask)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TokenLogprobsFn.apply(logits, labels, mask)
+    return _logprob_fwd(logits, labels, mask, False)[0]
+
+
+def _policy(logits, labels, mask, old, ref, adv, lo, hi, kl, want_grad):
+    B, L, V = logits.shape
+    dev = logits.device
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    lp, coef = (torch.empty(B, L, dtype=torch.float32, device=dev) for _ in range(2))
+    stats = d = None
+    if want_grad:
+        stats = torch.empty(B, L, 2, dtype=torch.float32, device=dev)
+        d = _grad_like(logits)
+    lib = N.lib()
+    nbytes = lib.mogt_policy_loss_scratch_bytes(B, L)
+    a_sb, a_sl = (adv.stride(0), 0) if adv.ndim == 1 else adv.stride()
+    with torch.cuda.device(dev):
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        N.check(lib.mogt_policy_loss(logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
+                                     _ptr(mask), old.data_ptr(), _ptr(ref), adv.data_ptr(), a_sb, a_sl, lo, hi, kl,
+                                     loss.data_ptr(), lp.data_ptr(), _ptr(stats), coef.data_ptr(), _ptr(d),
+                                     0 if d is None else d.stride(0), 0 if d is None else d.stride(1), B, L, V,
+                                     N.dtype_code(logits.dtype), scratch.data_ptr(), nbytes, _stream(dev)),
+                "mogt_policy_loss")
+    return loss, lp, stats, coef, d
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    """The forward also writes the gradient for d loss = 1 (the rows are on the
+    chip at that moment); the backward hands it out, scaled in place unless
+    the incoming gradient is 1.  A second backward (retain_graph) forms it
+    again from the logits, since the first one may have been changed by its
+    receiver."""
+
+    @staticmethod
+    def forward(ctx, logits, labels, mask, old, ref, adv, lo, hi, kl):
+        with torch.autograd.profiler.record_function("mogt.policy_loss.forward"):
+            loss, lp, stats, coef, d = _policy(logits, labels, mask, old, ref, adv, lo, hi, kl, True)
+        ctx.save_for_backward(logits, labels, mask, stats, coef)
+        ctx.grad = d
+        ctx.mark_non_differentiable(lp)
+        return loss, lp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _glp):
+        d, ctx.grad = ctx.grad, None
+        with torch.autograd.profiler.record_function("mogt.policy_loss.backward"):
+            if d is None:
+                logits, labels, mask, stats, coef = ctx.saved_tensors
+                d = _logprob_bwd(logits, labels, mask, stats, coef, 1, g)
+            else:
+                base = d if d.is_contiguous() else d._base
+                g = g.to(torch.float32).contiguous()
+                with torch.cuda.device(d.device):
+                    N.check(N.lib().mogt_scale_unless_one(base.data_ptr(), base.numel(), N.dtype_code(d.dtype),
+                                                          g.data_ptr(), _stream(d.device)), "mogt_scale_unless_one")
+        return (d,) + (None,) * 8
+
+
+def _token_f32(what, name, t, shape):
+    if t.shape != shape:
+        raise ValueError(f"{what}: {name} must be {list(shape)}")
+    return t.detach().to(torch.float32).contiguous()
+
+
+def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, mask=None, clip_low=0.2, clip_high=0.2,
+                kl_coef=0.0, return_logprobs=False):
+    """Clipped policy loss with a KL term, the mean over the counting tokens of
+
+        -min(r a, clip(r, 1 - clip_low, 1 + clip_high) a) + kl_coef (e^d - d - 1)
+
+    with lp = log softmax(logits)[label], r = exp(lp - old_logprobs),
+    d = ref_logprobs - lp and a the advantage.  old_logprobs, ref_logprobs:
+    [B, L] (the KL term needs ref_logprobs); advantages: [B] or [B, L].
+    Returns the loss (fp32 scalar), with ``return_logprobs`` also lp [B, L]."""
+    what = "policy_loss"
+    _cuda(what, logits, labels, old_logprobs, advantages, ref_logprobs, mask)
+    logits, labels, mask = _rows(what, logits, labels, mask)
+    shape = labels.shape
+    old = _token_f32(what, "old_logprobs", old_logprobs, shape)
+    if kl_coef != 0.0 and ref_logprobs is None:
+        raise ValueError(f"{what}: kl_coef needs ref_logprobs")
+    ref = None if ref_logprobs is None else _token_f32(what, "ref_logprobs", ref_logprobs, shape)
+    if advantages.shape not in (shape, shape[:1]):
+        raise ValueError(f"{what}: advantages must be [B] or [B, L]")
+    adv = advantages.detach().to(torch.float32)
+    if not (clip_low >= 0 and clip_high >= 0):
+        raise ValueError(f"{what}: clip_low and clip_high must not be negative")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        loss, lp = _PolicyLossFn.apply(logits, labels, mask, old, ref, adv, float(clip_low), float(clip_high),
+                                       float(kl_coef))
+    else:
+        with torch.autograd.profiler.record_function("mogt.policy_loss"):
+            loss, lp = _policy(logits, labels, mask, old, ref, adv, float(clip_low), float(clip_high), float(kl_coef),
+                               False)[:2]
+    return (loss, lp) if return_logprobs else loss
+
+
+def _preference(logits, labels, mask, ref, beta, eps, want_grad):
+    B, L, _ = logits.shape
+    dev = logits.device
+    lp, stats = _logprob_fwd(logits, labels, mask, want_grad)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    seq, coef = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
+    with torch.cuda.device(dev):
+        N.check(N.lib().mogt_preference_pairs(lp.data_ptr(), ref.data_ptr(), B // 2, L, beta, eps, loss.data_ptr(),
+                                              seq.data_ptr(), coef.data_ptr(), _stream(dev)), "mogt_preference_pairs")
+    return loss, seq, coef, stats
+
+
+class _PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, mask, ref, beta, eps):
+        with torch.autograd.profiler.record_function("mogt.preference_loss.forward"):
+            loss, seq, coef, stats = _preference(logits, labels, mask, ref, beta, eps, True)
+        ctx.save_for_backward(logits, labels, mask, stats, coef)
+        ctx.mark_non_differentiable(seq)
+        return loss, seq
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g, _gseq):
+        logits, labels, mask, stats, coef = ctx.saved_tensors
+        with torch.autograd.profiler.record_function("mogt.preference_loss.backward"):
+            d = _logprob_bwd(logits, labels, mask, stats, coef, max(logits.shape[1], 1), g)
+        return (d,) + (None,) * 5
+
+
+def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0.0, mask=None, return_logprobs=False):
+    """Paired preference loss.  Sequences 0..P-1 of the batch are preferred
+    over sequences P..2P-1.  With s the sum of a sequence's counting label
+    log-probabilities and ref_logprobs [2P] the reference model's sums,
+
+        x = beta ((s_p - ref_p) - (s_{P+p} - ref_{P+p}))
+        loss = mean_p [-(1 - eps) log sigmoid(x) - eps log sigmoid(-x)]
+
+    (eps = label_smoothing).  Returns the loss (fp32 scalar), with
+    ``return_logprobs`` also s [2P]."""
+    what = "preference_loss"
+    _cuda(what, logits, labels, ref_logprobs, mask)
+    logits, labels, mask = _rows(what, logits, labels, mask)
+    if logits.shape[0] % 2 or logits.shape[0] == 0:
+        raise ValueError(f"{what}: the batch must hold preferred sequences and as many others after them")
+    ref = _token_f32(what, "ref_logprobs", ref_logprobs, labels.shape[:1])
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"{what}: label_smoothing must lie in [0, 1]")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        loss, seq = _PreferenceLossFn.apply(logits, labels, mask, ref, float(beta), float(label_smoothing))
+    else:
+        with torch.autograd.profiler.record_function("mogt.preference_loss"):
+            loss, seq = _preference(logits, labels, mask, ref, float(beta), float(label_smoothing), False)[:2]
+    return (loss, seq) if return_logprobs else loss
