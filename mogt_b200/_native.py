@@ -134,6 +134,41 @@ def check(status: int, what: str) -> None:
     raise RuntimeError(f"{what}: {msg} (status {status})")
 
 
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call a C ABI function with `device`'s current stream as its last
+    argument, on that device, and check its status.  Plain integers for
+    pointers and no context manager when the device is already current: the
+    single-token calls are bound by the host, and this form costs a few
+    microseconds less than the ones below."""
+    fn = getattr(lib(), name)
+    index = device.index
+    if index == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if st != OK:
+        check(st, name)
+
+
+class tag:
+    """record_function(name) while a profiler runs, otherwise nothing."""
+    __slots__ = ("name", "rf")
+
+    def __init__(self, name):
+        self.name = name
+
+    def __enter__(self):
+        self.rf = None
+        if torch.autograd._profiler_enabled():
+            self.rf = torch.autograd.profiler.record_function(self.name)
+            self.rf.__enter__()
+
+    def __exit__(self, *exc):
+        if self.rf is not None:
+            self.rf.__exit__(*exc)
+
+
 def ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 

@@ -9,216 +9,440 @@
 // a_t h_{t-1} is kept as such (h_t - x_t B_t would cancel where a_t is small).
 //
 // The forward saved the state every 16 tokens.  A warp walks its channels'
-// tiles backwards; in a tile the first 8 tokens are stepped to get the state
-// in the middle, then each half is stepped again with a_t and a_t h_{t-1} of
-// its 8 tokens kept in registers, and walked backwards.  Lanes are those of
-// the forward (4 states each, LPC lanes per channel).  dB and dC need sums
-// over all channels: over the warp's by a halving butterfly that leaves each
-// lane one token, over the CTA's warps through shared memory, over CTAs by a
-// second kernel that adds the partial rows in a fixed order.  About 25
-// instructions per (token, channel, state), so instruction issue bounds it.
+// tiles backwards; a tile's first 12 tokens are stepped to get the states that
+// enter its groups of 4, then each group is stepped again with a_t and
+// a_t h_{t-1} kept in registers, and walked backwards.  Lanes are those of
+// the forward (4 states each, LPC lanes per channel), and a long sequence is
+// split into segments as there, the adjoint's carries from a first pass.
+//
+// dB and dC need sums over all channels.  Per token a lane holds 8 terms (4
+// states of each), the warp's channels are added by halving exchanges that
+// leave a lane one term: a lane keeps its states in an order XORed with its
+// channel number (B and C come in as many permuted copies), so that what it
+// sends is always the same registers and no selects are needed.  The CTA's
+// warps add through shared memory and CTAs through a second kernel, in a
+// fixed order.  Instruction issue bounds it (about 20 per token, channel and
+// state), then the shuffles.
 #include "selective_scan.cuh"
 
 namespace mogt {
 namespace sel {
 
+#ifndef MOGT_BWD_WARPS
+#define MOGT_BWD_WARPS 16
+#endif
+#ifndef MOGT_BWD_CTAS
+#define MOGT_BWD_CTAS 2
+#endif
+constexpr int kBwdWarps = MOGT_BWD_WARPS;  // warps per SM that the backward asks for
+
 struct BwdScratch {
+  SegScratch seg;
   float* bc;   // [nblk][B][G][L][2][NP]
-  float* dA;   // [B][D][NP]
-  float* dv;   // [B][2][D]: dD, dbias
+  float* dA;   // [nseg * B][D][NP]
+  float* dv;   // [nseg * B][2][D]: dD, dbias
 };
+
+// States in XORed order: slot i of a lane of channel c holds state i ^ (c & mask).
+template <int LPC>
+struct Perm {
+  static constexpr int COPIES = Lane<LPC>::CPW >= 4 ? 4 : Lane<LPC>::CPW;
+  static constexpr int MASK = COPIES - 1;
+  __device__ static __forceinline__ float4 apply(float4 v, int c) {
+    if (COPIES > 1 && (c & 1)) v = make_float4(v.y, v.x, v.w, v.z);
+    if (COPIES > 2 && (c & 2)) v = make_float4(v.z, v.w, v.x, v.y);
+    return v;
+  }
+};
+
+// One token's B or C: for every 4 states their COPIES orders side by side, so
+// that the lanes of a quarter warp (one part, 8 channels) read 64 consecutive
+// bytes: [part][copy][4].
+template <typename T, int LPC, int THREADS>
+__device__ __forceinline__ void put_copies(float4 (*dst)[LPC][Perm<LPC>::COPIES],
+                                           const BcRaw<T, Lane<LPC>::NP, THREADS>& r, int N, int last) {
+  constexpr int NP = Lane<LPC>::NP;
+#pragma unroll
+  for (int x = 0; x < BcRaw<T, NP, THREADS>::PER; ++x) {
+    const int i = threadIdx.x + x * THREADS;
+    if (kTile * NP % THREADS == 0 || i < kTile * NP) {
+      const int k = i / NP, n = i % NP;
+      const float v = r.get(x, N, last);
+#pragma unroll
+      for (int q = 0; q < Perm<LPC>::COPIES; ++q) reinterpret_cast<float*>(&dst[k][n / NS][q])[(n % NS) ^ q] = v;
+    }
+  }
+}
 
 template <int LPC>
 struct BwdSmem {
-  float B[kTile][Lane<LPC>::NP], C[kTile][Lane<LPC>::NP];
-  float4 stage[NTB / 32][kTile][Lane<LPC>::CPW];
-  float red[NTB / 32][kGroup][2][Lane<LPC>::NP];
+  float4 B[2][kTile][LPC][Perm<LPC>::COPIES], C[2][kTile][LPC][Perm<LPC>::COPIES];
+  float2 s1[NTB / 32][kTile][Lane<LPC>::CPW];   // (dt, x)
+  float4 s2[NTB / 32][kTile][Lane<LPC>::CPW];   // (dy, u, softplus', dout silu'(z))
+  float red[2][NTB / 32][kGroupB][2][Lane<LPC>::NP];
 };
 
+// First pass over a split sequence: per segment (all but the first) the
+// adjoint handed to the state before it, from nothing behind it, and sum dt.
 template <typename T, int LPC>
-__global__ void __launch_bounds__(NTB) scan_bwd_kernel(const mogt_selective_args p, const Geo geo,
-                                                       const BwdScratch sc) {
+__global__ void __launch_bounds__(NT, LPC < 4 ? 3 : 4) scan_bwd_agg_kernel(const mogt_selective_args p,
+                                                                         const Geo geo, const SegScratch seg) {
   using Q = Lane<LPC>;
   constexpr int CPW = Q::CPW, TPL = Q::TPL, NP = Q::NP;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  BwdSmem<LPC>& sm = *reinterpret_cast<BwdSmem<LPC>*>(smem_raw);
+  __shared__ __align__(16) float sC[2][kTile][NP];
+  __shared__ float2 stage[NT / 32][kTile][CPW];  // (dt, dy)
   const Where<LPC> w(p, geo);
   const int64_t len = seq_len(p.lengths, w.b, p.L);
-
-  float A2[NS], carry[NS], accA[NS];
+  const int64_t k0 = (int64_t)(blockIdx.y + 1) * geo.tps, k1 = min(k0 + geo.tps, geo.nck);
+  const int64_t kl = min(k1, (len + kTile - 1) / kTile);
+  const int64_t cell = w.b * p.D + w.d;
+  float A2[NS];
   load_A<LPC>(A2, p, w);
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    const int n = w.j * NS + i;
-    carry[i] = (p.dfinal && w.ok && n < p.N) ? p.dfinal[(w.b * p.D + w.d) * p.N + n] : 0.f;
-    accA[i] = 0.f;
-  }
-  const float Dd = p.Dskip && w.ok ? p.Dskip[w.d] : 0.f;
-  const float bias = p.bias && w.ok ? p.bias[w.d] : 0.f;
-  float accD = 0.f, accb = 0.f;
-  const float4* saved = reinterpret_cast<const float4*>(p.saved);
-  T* du = static_cast<T*>(p.du) + w.b * p.L * p.D + w.d;
-  T* ddelta = static_cast<T*>(p.ddelta) + w.b * p.L * p.D + w.d;
-  T* dz = p.z ? static_cast<T*>(p.dz) + w.b * p.L * p.D + w.d : nullptr;
-
-  for (int64_t tile = geo.nck - 1; tile >= 0; --tile) {
-    const int64_t t0 = tile * kTile;
-    if (t0 >= len) {
-      for (int k = w.part_tok(); k < kTile; k += kGroup)
-#pragma unroll
-        for (int i = 0; i < TPL; ++i) {
-          const int64_t t = t0 + k + i;
-          if (w.ok && w.owner() && t < p.L) {
-            du[t * p.D] = from_f32<T>(0.f);
-            ddelta[t * p.D] = from_f32<T>(0.f);
-            if (dz) dz[t * p.D] = from_f32<T>(0.f);
-          }
-        }
-      continue;
-    }
-    __syncthreads();
-    load_bc<T, NP>(sm.B, p, w, static_cast<const T*>(p.Bm), p.B_sb, p.B_sl, p.B_sg, t0, len);
-    load_bc<T, NP>(sm.C, p, w, static_cast<const T*>(p.Cm), p.C_sb, p.C_sl, p.C_sg, t0, len);
-    float u[2][TPL], raw[2][TPL], z[2][TPL], go[2][TPL];
+  const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
+  F2 g01 = 0, g23 = 0;
+  const float bias = p.bias ? p.bias[w.d] : 0.f;
+  const int tok = w.part_tok(), N = (int)p.N;
+  const int d_sl = (int)p.delta_sl, z_sl = (int)p.z_sl, o_sl = (int)p.dout_sl, C_sl = (int)p.C_sl;
+  const bool gate = p.z, sp = p.softplus;
+  const T* dp = static_cast<const T*>(p.delta) + w.b * p.delta_sb + w.d;
+  const T* zp = static_cast<const T*>(p.z) + w.b * p.z_sb + w.d;
+  const T* op = static_cast<const T*>(p.dout) + w.b * p.dout_sb + w.d;
+  const T* Cp = static_cast<const T*>(p.Cm) + w.b * p.C_sb + w.g * p.C_sg;
+  TileRaw<T, TPL, kGroup> rd, rz, ro;
+  BcRaw<T, NP, NT> rC;
+  int last = 0;
+  auto fetch = [&](int64_t k) {
+    const int64_t t0 = k * kTile;
+    last = (int)min(len - 1 - t0, (int64_t)(kTile - 1));
+    rC.fetch(Cp + t0 * C_sl, C_sl, N, last);
+    rd.fetch(dp + t0 * d_sl, d_sl, tok, last);
+    ro.fetch(op + t0 * o_sl, o_sl, tok, last);
+    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, tok, last);
+  };
+  float sdt = 0.f;
+  if (k0 < kl) fetch(kl - 1);
+  for (int64_t k = kl - 1; k >= k0; --k) {
+    const int buf = (int)(k & 1), live = last;
+    rC.put(sC[buf], N, live);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int i = 0; i < TPL; ++i) {
-        const int64_t t = t0 + q * kGroup + w.part_tok() + i;
-        float dt = 0.f;
-        u[q][i] = raw[q][i] = z[q][i] = go[q][i] = 0.f;
-        if (w.ok && t < len) {
-          u[q][i] = to_f32(static_cast<const T*>(p.u)[w.b * p.u_sb + t * p.u_sl + w.d]);
-          raw[q][i] = dt = to_f32(static_cast<const T*>(p.delta)[w.b * p.delta_sb + t * p.delta_sl + w.d]) + bias;
-          if (p.softplus) dt = softplus(dt);
-          go[q][i] = to_f32(static_cast<const T*>(p.dout)[w.b * p.dout_sb + t * p.dout_sl + w.d]);
-          if (p.z) z[q][i] = to_f32(static_cast<const T*>(p.z)[w.b * p.z_sb + t * p.z_sl + w.d]);
+        const int kk = q * kGroup + tok + i;
+        float dt = to_f32(rd.v[q][i]) + bias, dy = to_f32(ro.v[q][i]);
+        if (sp) dt = softplus(dt);
+        if (gate) {
+          const float z = to_f32(rz.v[q][i]);
+          dy *= z * sigmoid(z);
         }
-        const float dy = p.z ? go[q][i] * z[q][i] * sigmoid(z[q][i]) : go[q][i];
-        if (w.owner())
-          sm.stage[w.warp][q * kGroup + w.part_tok() + i][w.c] = make_float4(dt, dt * u[q][i], dy, 0.f);
+        if (kk > live) dt = dy = 0.f;
+        if (Q::DUP == 1 || w.owner()) stage[w.warp][kk][w.c] = make_float2(dt, dy);
       }
     __syncthreads();
-    float h0[NS], hm[NS];
-    {
-      const float4 v = w.ok ? saved[((w.b * geo.nck + tile) * p.D + w.d) * LPC + w.j] : make_float4(0, 0, 0, 0);
-      h0[0] = v.x; h0[1] = v.y; h0[2] = v.z; h0[3] = v.w;
+    if (k > k0) fetch(k - 1);
+    float sd = 0.f;
+#pragma unroll
+    for (int kk = kTile - 1; kk >= 0; --kk) {
+      const float2 s = stage[w.warp][kk][w.c];
+      const F2 dt2 = f2(s.x, s.x), dy2 = f2(s.y, s.y);
+      const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(&sC[buf][kk][w.j * NS]);
+      g01 = mul2(exp2_2(mul2(dt2, A01)), fma2(Cv.x, dy2, g01));
+      g23 = mul2(exp2_2(mul2(dt2, A23)), fma2(Cv.y, dy2, g23));
+      sd += s.x;
     }
-#pragma unroll
-    for (int i = 0; i < NS; ++i) hm[i] = h0[i];
-    if (t0 + kGroup < len) {
-#pragma unroll
-      for (int k = 0; k < kGroup; ++k) {
-        const float4 s = sm.stage[w.warp][k][w.c];
-#pragma unroll
-        for (int i = 0; i < NS; ++i)
-          hm[i] = fmaf(fast_exp2(s.x * A2[i]), hm[i], s.y * sm.B[k][w.j * NS + i]);
-      }
-    }
-#pragma unroll 1
-    for (int q = 1; q >= 0; --q) {
-      float a[kGroup][NS], ph[kGroup][NS], h[NS];
-#pragma unroll
-      for (int i = 0; i < NS; ++i) h[i] = q ? hm[i] : h0[i];
-#pragma unroll
-      for (int k = 0; k < kGroup; ++k) {
-        const float4 s = sm.stage[w.warp][q * kGroup + k][w.c];
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          a[k][i] = fast_exp2(s.x * A2[i]);
-          ph[k][i] = a[k][i] * h[i];
-          h[i] = fmaf(s.y, sm.B[q * kGroup + k][w.j * NS + i], ph[k][i]);
-        }
-      }
-      float ysw[kGroup][3], bc[kGroup][2 * NS];
-#pragma unroll
-      for (int k = kGroup - 1; k >= 0; --k) {
-        const float4 s = sm.stage[w.warp][q * kGroup + k][w.c];
-        float y = 0.f, ss = 0.f, ww = 0.f;
-#pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          const float Bn = sm.B[q * kGroup + k][w.j * NS + i], Cn = sm.C[q * kGroup + k][w.j * NS + i];
-          const float hk = fmaf(s.y, Bn, ph[k][i]);
-          const float g = fmaf(Cn, s.z, carry[i]);
-          y = fmaf(Cn, hk, y);
-          bc[k][i] = g * s.y;
-          bc[k][NS + i] = s.z * hk;
-          ss = fmaf(g, Bn, ss);
-          const float qq = g * ph[k][i];
-          ww = fmaf(A2[i], qq, ww);
-          accA[i] = fmaf(s.x, qq, accA[i]);
-          carry[i] = a[k][i] * g;
-        }
-        ysw[k][0] = y;
-        ysw[k][1] = ss;
-        ysw[k][2] = ww;
-      }
-      sum_parts<LPC, 3>(ysw, w.j);
-      sum_channels<CPW, 2 * NS>(bc, w.c);
-      using CT = ChanTok<CPW>;
-      if (CT::owner(w.c)) {
-#pragma unroll
-        for (int i = 0; i < CT::TPL; ++i) {
-          float(*r)[NP] = sm.red[w.warp][CT::first(w.c) + i];
-          *reinterpret_cast<float4*>(&r[0][w.j * NS]) = make_float4(bc[i][0], bc[i][1], bc[i][2], bc[i][3]);
-          *reinterpret_cast<float4*>(&r[1][w.j * NS]) = make_float4(bc[i][4], bc[i][5], bc[i][6], bc[i][7]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < TPL; ++i) {
-        const int kk = w.part_tok() + i;
-        const int64_t t = t0 + q * kGroup + kk;
-        const float uu = q ? u[1][i] : u[0][i], rr = q ? raw[1][i] : raw[0][i];
-        const float zz = q ? z[1][i] : z[0][i], gg = q ? go[1][i] : go[0][i];
-        const float4 s = sm.stage[w.warp][q * kGroup + kk][w.c];
-        const float gu = fmaf(s.x, ysw[i][1], Dd * s.z);
-        float gd = fmaf(uu, ysw[i][1], kLn2 * ysw[i][2]);
-        if (p.softplus) gd *= sigmoid(rr);
-        if (w.ok && w.owner() && t < p.L) {
-          const bool live = t < len;
-          du[t * p.D] = from_f32<T>(live ? gu : 0.f);
-          ddelta[t * p.D] = from_f32<T>(live ? gd : 0.f);
-          if (dz) {
-            const float sg = sigmoid(zz), yt = fmaf(Dd, uu, ysw[i][0]);
-            dz[t * p.D] = from_f32<T>(live ? gg * yt * sg * (1.f + zz * (1.f - sg)) : 0.f);
-          }
-          if (live) {
-            accD = fmaf(s.z, uu, accD);
-            accb += gd;
-          }
-        }
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < kGroup * 2 * NP; i += NTB) {
-        float v = 0.f;
-#pragma unroll
-        for (int ww = 0; ww < NTB / 32; ++ww) v += (&sm.red[ww][0][0][0])[i];
-        const int64_t t = t0 + q * kGroup + i / (2 * NP);
-        if (t < len)
-          sc.bc[((((blockIdx.x % geo.nblk) * p.B + w.b) * p.G + w.g) * p.L + t) * (2 * NP) + i % (2 * NP)] = v;
-      }
-      __syncthreads();
-    }
+    sdt += sd;
+    __syncwarp();
   }
   if (w.ok) {
-    *reinterpret_cast<float4*>(sc.dA + ((w.b * p.D + w.d) * LPC + w.j) * NS) =
-        make_float4(accA[0], accA[1], accA[2], accA[3]);
-    if (p.dinit) {
+    const float2 a = un2(g01), b = un2(g23);
+    const int64_t i = blockIdx.y * p.B * p.D + cell;
+    seg.loc[i * LPC + w.j] = make_float4(a.x, a.y, b.x, b.y);
+    if (w.j == 0) seg.sdt[i] = sdt;
+  }
+}
+
+// Sums the 8 terms of one token (dB: v[0..3], dC: v[4..7], XORed order) over
+// the warp's channels and leaves them in row r[2][NP] of shared memory.
+template <int LPC>
+__device__ __forceinline__ void channel_sums(F2 b01, F2 b23, F2 c01, F2 c23, float (*r)[Lane<LPC>::NP], int c,
+                                             int j) {
+  constexpr int CPW = Lane<LPC>::CPW;
+  constexpr unsigned ALL = 0xffffffffu;
+  const float2 b0 = un2(b01), b1 = un2(b23), c0 = un2(c01), c1 = un2(c23);
+  float v[8] = {b0.x, b0.y, b1.x, b1.y, c0.x, c0.y, c1.x, c1.y};
+  const int n0 = j * NS;
+  if constexpr (CPW == 1) {
+    *reinterpret_cast<float4*>(&r[0][n0]) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4*>(&r[1][n0]) = make_float4(v[4], v[5], v[6], v[7]);
+  } else if constexpr (CPW == 2) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const int n = w.j * NS + i;
-        if (n < p.N) p.dinit[(w.b * p.D + w.d) * p.N + n] = carry[i];
+    for (int i = 0; i < 8; i += 2) v[i] += __shfl_xor_sync(ALL, v[i + 1], 1);
+    r[0][n0 + c] = v[0];
+    r[0][n0 + 2 + c] = v[2];
+    r[1][n0 + c] = v[4];
+    r[1][n0 + 2 + c] = v[6];
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; q += 4) {
+      v[q] += __shfl_xor_sync(ALL, v[q + 2], 2);
+      v[q + 1] += __shfl_xor_sync(ALL, v[q + 3], 2);
+      v[q] += __shfl_xor_sync(ALL, v[q + 1], 1);
+    }
+    if constexpr (CPW == 4) {
+      r[0][n0 + c] = v[0];
+      r[1][n0 + c] = v[4];
+    } else {
+      const bool hi = c & 4;
+      float t = (hi ? v[4] : v[0]) + __shfl_xor_sync(ALL, hi ? v[0] : v[4], 4);
+      if constexpr (CPW >= 16) t += __shfl_xor_sync(ALL, t, 8);
+      if constexpr (CPW >= 32) t += __shfl_xor_sync(ALL, t, 16);
+      if (CPW == 8 || c < 8) r[hi ? 1 : 0][n0 + (c & 3)] = t;
+    }
+  }
+}
+
+template <typename T, int LPC>
+__global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
+    scan_bwd_kernel(const mogt_selective_args p, const Geo geo, const BwdScratch sc) {
+  using Q = Lane<LPC, kGroupB>;
+  constexpr int CPW = Q::CPW, TPL = Q::TPL, NP = Q::NP, NG = kTile / kGroupB;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  BwdSmem<LPC>& sm = *reinterpret_cast<BwdSmem<LPC>*>(smem_raw);
+  const Where<LPC, kGroupB> w(p, geo);
+  const int64_t len = seq_len(p.lengths, w.b, p.L);
+  const int64_t k0 = (int64_t)blockIdx.y * geo.tps, k1 = min(k0 + geo.tps, geo.nck);
+  const int64_t kl = min(k1, (len + kTile - 1) / kTile);
+  const int64_t cell = w.b * p.D + w.d;
+  const int cq = w.c & Perm<LPC>::MASK;
+
+  F2 A01, A23, cy01, cy23;
+  {
+    float A2[NS], cy[NS];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int n = w.j * NS + (i ^ cq);
+      A2[i] = (w.ok && n < p.N) ? p.A[w.d * p.N + n] * kLog2e : 0.f;
+      cy[i] = (p.dfinal && w.ok && n < p.N) ? p.dfinal[cell * p.N + n] : 0.f;
+    }
+#pragma unroll 4
+    for (int s = geo.nseg - 1; s > (int)blockIdx.y; --s) {
+      const int64_t i = (s - 1) * p.B * p.D + cell;
+      const float4 l = Perm<LPC>::apply(sc.seg.loc[i * LPC + w.j], w.c);
+      const float sd = sc.seg.sdt[i];
+      cy[0] = fmaf(fast_exp2(sd * A2[0]), cy[0], l.x);
+      cy[1] = fmaf(fast_exp2(sd * A2[1]), cy[1], l.y);
+      cy[2] = fmaf(fast_exp2(sd * A2[2]), cy[2], l.z);
+      cy[3] = fmaf(fast_exp2(sd * A2[3]), cy[3], l.w);
+    }
+    A01 = f2(A2[0], A2[1]);
+    A23 = f2(A2[2], A2[3]);
+    cy01 = f2(cy[0], cy[1]);
+    cy23 = f2(cy[2], cy[3]);
+  }
+  const F2 one = f2(1.f, 1.f);
+  F2 sumA01 = 0, sumA23 = 0;
+  float sumD = 0.f, sumb = 0.f;
+  const float Dd = p.Dskip ? p.Dskip[w.d] : 0.f;
+  const float bias = p.bias ? p.bias[w.d] : 0.f;
+  const bool gate = p.z, sp = p.softplus, store = w.ok && w.owner();
+  const int tok = w.part_tok(), N = (int)p.N, D = (int)p.D;
+  const int u_sl = (int)p.u_sl, d_sl = (int)p.delta_sl, z_sl = (int)p.z_sl, o_sl = (int)p.dout_sl,
+            B_sl = (int)p.B_sl, C_sl = (int)p.C_sl;
+  const T* up = static_cast<const T*>(p.u) + w.b * p.u_sb + w.d;
+  const T* dp = static_cast<const T*>(p.delta) + w.b * p.delta_sb + w.d;
+  const T* zp = static_cast<const T*>(p.z) + w.b * p.z_sb + w.d;
+  const T* op = static_cast<const T*>(p.dout) + w.b * p.dout_sb + w.d;
+  const T* Bp = static_cast<const T*>(p.Bm) + w.b * p.B_sb + w.g * p.B_sg;
+  const T* Cp = static_cast<const T*>(p.Cm) + w.b * p.C_sb + w.g * p.C_sg;
+  const float4* saved = reinterpret_cast<const float4*>(p.saved) + (w.b * geo.nck * p.D + w.d) * LPC + w.j;
+  const int64_t o0 = (w.b * p.L + tok) * p.D + w.d;
+  T* du = static_cast<T*>(p.du) + o0;
+  T* ddelta = static_cast<T*>(p.ddelta) + o0;
+  T* dz = gate ? static_cast<T*>(p.dz) + o0 : nullptr;
+  float* bcp = sc.bc + (((blockIdx.x % geo.nblk) * p.B + w.b) * p.G + w.g) * p.L * (2 * NP);
+
+  // tiles behind the end
+  for (int64_t t = max(kl, k0) * kTile; t < min(k1 * kTile, p.L); t += kGroupB)
+#pragma unroll
+    for (int i = 0; i < TPL; ++i)
+      if (store && t + tok + i < p.L) {
+        du[(t + i) * p.D] = from_f32<T>(0.f);
+        ddelta[(t + i) * p.D] = from_f32<T>(0.f);
+        if (gate) dz[(t + i) * p.D] = from_f32<T>(0.f);
       }
+
+  TileRaw<T, TPL, kGroupB> ru, rd, rz, ro;
+  BcRaw<T, NP, NTB> rB, rC;
+  float4 rs;
+  int last = 0;
+  auto fetch = [&](int64_t k) {
+    const int64_t t0 = k * kTile;
+    last = (int)min(len - 1 - t0, (int64_t)(kTile - 1));
+    rB.fetch(Bp + t0 * B_sl, B_sl, N, last);
+    rC.fetch(Cp + t0 * C_sl, C_sl, N, last);
+    rd.fetch(dp + t0 * d_sl, d_sl, tok, last);
+    ru.fetch(up + t0 * u_sl, u_sl, tok, last);
+    ro.fetch(op + t0 * o_sl, o_sl, tok, last);
+    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, tok, last);
+    rs = saved[k * p.D * LPC];
+  };
+  if (k0 < kl) fetch(kl - 1);
+  for (int64_t k = kl - 1; k >= k0; --k) {
+    const int64_t t0 = k * kTile;
+    const int buf = (int)(k & 1), live = last;
+    put_copies<T, LPC, NTB>(sm.B[buf], rB, N, live);
+    put_copies<T, LPC, NTB>(sm.C[buf], rC, N, live);
+#pragma unroll
+    for (int q = 0; q < NG; ++q)
+#pragma unroll
+      for (int i = 0; i < TPL; ++i) {
+        const int kk = q * kGroupB + tok + i;
+        const float u = to_f32(ru.v[q][i]);
+        float dt = to_f32(rd.v[q][i]) + bias, dy = to_f32(ro.v[q][i]), ds = 1.f, zf = 0.f;
+        if (sp) {
+          const float e = exp_neg_abs(dt);
+          ds = __fdividef(dt >= 0.f ? 1.f : e, 1.f + e);
+          dt = softplus_e(dt, e);
+        }
+        if (gate) {
+          const float z = to_f32(rz.v[q][i]), sg = sigmoid(z);
+          zf = dy * sg * (1.f + z * (1.f - sg));
+          dy *= z * sg;
+        }
+        float x = dt * u;
+        // dead tokens, and lanes without a channel (they share the sums over channels)
+        if (kk > live || !w.ok) dt = x = dy = 0.f;
+        if (Q::DUP == 1 || w.owner()) {
+          sm.s1[w.warp][kk][w.c] = make_float2(dt, x);
+          sm.s2[w.warp][kk][w.c] = make_float4(dy, u, ds, zf);
+        }
+      }
+    float4 h0 = Perm<LPC>::apply(rs, w.c);
+    if (!w.ok) h0 = make_float4(0.f, 0.f, 0.f, 0.f);
+    __syncthreads();
+    if (k > k0) fetch(k - 1);
+    // states entering the tile's groups
+    F2 hs[NG][2];
+    hs[0][0] = f2(h0.x, h0.y);
+    hs[0][1] = f2(h0.z, h0.w);
+#pragma unroll
+    for (int q = 0; q + 1 < NG; ++q) {
+      F2 h01 = hs[q][0], h23 = hs[q][1];
+#pragma unroll
+      for (int i = 0; i < kGroupB; ++i) {
+        const int kk = q * kGroupB + i;
+        const float2 s = sm.s1[w.warp][kk][w.c];
+        const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y);
+        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
+        h01 = fma2(exp2_2(mul2(dt2, A01)), h01, mul2(x2, Bv.x));
+        h23 = fma2(exp2_2(mul2(dt2, A23)), h23, mul2(x2, Bv.y));
+      }
+      hs[q + 1][0] = h01;
+      hs[q + 1][1] = h23;
+    }
+    F2 tA01 = 0, tA23 = 0;
+    float tD = 0.f, tb = 0.f;
+    const int rows = (int)min(p.L - t0, (int64_t)kTile);
+#pragma unroll
+    for (int q = NG - 1; q >= 0; --q) {
+      F2 a[kGroupB][2], ph[kGroupB][2];
+      F2 h01 = hs[q][0], h23 = hs[q][1];
+#pragma unroll
+      for (int i = 0; i < kGroupB; ++i) {
+        const int kk = q * kGroupB + i;
+        const float2 s = sm.s1[w.warp][kk][w.c];
+        const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y);
+        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
+        a[i][0] = exp2_2(mul2(dt2, A01));
+        a[i][1] = exp2_2(mul2(dt2, A23));
+        ph[i][0] = mul2(a[i][0], h01);
+        ph[i][1] = mul2(a[i][1], h23);
+        h01 = fma2(x2, Bv.x, ph[i][0]);
+        h23 = fma2(x2, Bv.y, ph[i][1]);
+      }
+      float ysw[kGroupB][3];
+#pragma unroll
+      for (int i = kGroupB - 1; i >= 0; --i) {
+        const int kk = q * kGroupB + i;
+        const float2 s = sm.s1[w.warp][kk][w.c];
+        const float dyv = sm.s2[w.warp][kk][w.c].x;
+        const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y), dy2 = f2(dyv, dyv);
+        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
+        const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(&sm.C[buf][kk][w.j][cq]);
+        h01 = fma2(x2, Bv.x, ph[i][0]);
+        h23 = fma2(x2, Bv.y, ph[i][1]);
+        const F2 g01 = fma2(Cv.x, dy2, cy01), g23 = fma2(Cv.y, dy2, cy23);
+        const F2 q01 = mul2(g01, ph[i][0]), q23 = mul2(g23, ph[i][1]);
+        ysw[i][0] = hsum(fma2(Cv.y, h23, mul2(Cv.x, h01)));
+        ysw[i][1] = hsum(fma2(Bv.y, g23, mul2(Bv.x, g01)));
+        ysw[i][2] = hsum(fma2(A23, q23, mul2(A01, q01)));
+        tA01 = fma2(dt2, q01, tA01);
+        tA23 = fma2(dt2, q23, tA23);
+        cy01 = mul2(a[i][0], g01);
+        cy23 = mul2(a[i][1], g23);
+        channel_sums<LPC>(mul2(g01, x2), mul2(g23, x2), mul2(dy2, h01), mul2(dy2, h23), sm.red[q & 1][w.warp][i], w.c,
+                          w.j);
+      }
+      sum_parts<LPC>(ysw, w.j);
+#pragma unroll
+      for (int i = 0; i < TPL; ++i) {
+        const int kk = q * kGroupB + i;  // + tok
+        const float dt = sm.s1[w.warp][kk + tok][w.c].x;
+        const float4 s2 = sm.s2[w.warp][kk + tok][w.c];  // (dy, u, softplus', dout silu'(z))
+        float gu = fmaf(dt, ysw[i][1], Dd * s2.x);
+        float gd = fmaf(s2.y, ysw[i][1], kLn2 * ysw[i][2]) * s2.z;
+        float gz = s2.w * fmaf(Dd, s2.y, ysw[i][0]);
+        if (kk + tok > live) {
+          gu = gd = gz = 0.f;
+        } else {
+          tD = fmaf(s2.x, s2.y, tD);
+          tb += gd;
+        }
+        if (store && kk + tok < rows) {
+          const int64_t o = (t0 + kk) * D;
+          du[o] = from_f32<T>(gu);
+          ddelta[o] = from_f32<T>(gd);
+          if (gate) dz[o] = from_f32<T>(gz);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i0 = 0; i0 < kGroupB * 2 * NP; i0 += NTB) {
+        const int i = i0 + threadIdx.x;
+        if (kGroupB * 2 * NP % NTB == 0 || i < kGroupB * 2 * NP) {
+          float v = 0.f;
+#pragma unroll
+          for (int ww = 0; ww < NTB / 32; ++ww) v += (&sm.red[q & 1][ww][0][0][0])[i];
+          const int kk = q * kGroupB + i / (2 * NP);
+          if (kk <= live) bcp[(t0 + kk) * (2 * NP) + i % (2 * NP)] = v;
+        }
+      }
+    }
+    sumA01 = fma2(one, tA01, sumA01);
+    sumA23 = fma2(one, tA23, sumA23);
+    sumD += tD;
+    sumb += tb;
+  }
+  if (!w.owner()) sumD = sumb = 0.f;
+  const int64_t row = blockIdx.y * p.B + w.b;
+  if (w.ok) {
+    const float2 a0 = un2(sumA01), a1 = un2(sumA23), c0 = un2(cy01), c1 = un2(cy23);
+    const float sa[NS] = {a0.x, a0.y, a1.x, a1.y}, cc[NS] = {c0.x, c0.y, c1.x, c1.y};
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+      const int n = w.j * NS + (i ^ cq);
+      sc.dA[(row * p.D + w.d) * NP + n] = sa[i];
+      if (p.dinit && blockIdx.y == 0 && n < p.N) p.dinit[cell * p.N + n] = cc[i];
     }
   }
 #pragma unroll
   for (int o = CPW; o < 32; o <<= 1) {
-    accD += __shfl_xor_sync(0xffffffffu, accD, o);
-    accb += __shfl_xor_sync(0xffffffffu, accb, o);
+    sumD += __shfl_xor_sync(0xffffffffu, sumD, o);
+    sumb += __shfl_xor_sync(0xffffffffu, sumb, o);
   }
   if (w.ok && w.j == 0) {
-    sc.dv[(w.b * 2 + 0) * p.D + w.d] = accD;
-    sc.dv[(w.b * 2 + 1) * p.D + w.d] = accb;
+    sc.dv[(row * 2 + 0) * p.D + w.d] = sumD;
+    sc.dv[(row * 2 + 1) * p.D + w.d] = sumb;
   }
 }
 
@@ -241,28 +465,29 @@ __global__ void __launch_bounds__(256) reduce_bc_kernel(const mogt_selective_arg
   dst[(bt * p.G + g) * p.N + n] = from_f32<T>(v);
 }
 
-// dA, dD, dbias from the per-sequence partial sums.
+// dA, dD, dbias from the partial sums of sequences and segments.
 __global__ void __launch_bounds__(256) reduce_param_kernel(const mogt_selective_args p, int NP, int64_t rows,
                                                            const BwdScratch sc) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t na = p.D * p.N;
   if (i < na) {
     const int64_t d = i / p.N, n = i % p.N;
-    float v = 0.f;
+    double v = 0.0;
     for (int64_t r = 0; r < rows; ++r) v += sc.dA[(r * p.D + d) * NP + n];
-    p.dA[i] = v;
+    p.dA[i] = (float)v;
   } else if (i < na + 2 * p.D) {
     const int64_t k = i - na;
-    float v = 0.f;
+    double v = 0.0;
     for (int64_t r = 0; r < rows; ++r) v += sc.dv[r * 2 * p.D + k];
     float* dst = k < p.D ? p.dD : p.dbias;
-    if (dst) dst[k % p.D] = v;
+    if (dst) dst[k % p.D] = (float)v;
   }
 }
 
-inline int64_t bc_floats(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
-  const int64_t cpb = NTB / lpc_of(N);
-  return (D / G + cpb - 1) / cpb * B * G * L * 2 * lpc_of(N) * NS;
+inline size_t bwd_floats(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G, int64_t nseg) {
+  const int64_t np = lpc_of(N) * NS, cpb = NTB / lpc_of(N);
+  const int64_t seg = (int64_t)(seg_scratch_bytes(B, D, N, nseg) / sizeof(float) + 3) / 4 * 4;
+  return (size_t)(seg + (D / G + cpb - 1) / cpb * B * G * L * 2 * np + nseg * B * D * (np + 2));
 }
 
 }  // namespace sel
@@ -273,7 +498,7 @@ using namespace mogt::sel;
 
 extern "C" size_t mogt_selective_bwd_scratch_bytes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
   if (B <= 0 || L < 0 || D <= 0 || N <= 0 || N > kMaxN || G <= 0 || D % G) return 0;
-  return (size_t)(bc_floats(B, L, D, N, G) + B * D * (lpc_of(N) * NS + 2)) * sizeof(float);
+  return bwd_floats(B, L, D, N, G, num_segments(B, L, D, N, G, NTB, kBwdWarps)) * sizeof(float);
 }
 
 extern "C" int mogt_selective_scan_bwd(const mogt_selective_args* args, void* stream) {
@@ -288,26 +513,32 @@ extern "C" int mogt_selective_scan_bwd(const mogt_selective_args* args, void* st
   if (!p.scratch || p.scratch_bytes < mogt_selective_bwd_scratch_bytes(p.B, p.L, p.D, p.N, p.G))
     return MOGT_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(p.scratch) | reinterpret_cast<uintptr_t>(p.saved)) & 15u) return MOGT_ERR_ALIGN;
-  const Geo geo = geometry(p, NTB);
+  const Geo geo = geometry(p, NTB, kBwdWarps);
   const int NP = lpc_of(p.N) * NS;
   BwdScratch sc;
-  sc.dA = static_cast<float*>(p.scratch);
-  sc.dv = sc.dA + p.B * p.D * NP;
-  sc.bc = sc.dv + 2 * p.B * p.D;
+  sc.seg = seg_scratch(p.scratch, p.B, p.D, p.N, geo.nseg);
+  sc.dA = static_cast<float*>(p.scratch) + (seg_scratch_bytes(p.B, p.D, p.N, geo.nseg) / sizeof(float) + 3) / 4 * 4;
+  sc.dv = sc.dA + geo.nseg * p.B * p.D * NP;
+  sc.bc = sc.dv + geo.nseg * p.B * 2 * p.D;
   cudaStream_t s = (cudaStream_t)stream;
-  const dim3 grid((unsigned)(geo.nblk * p.G), 1, (unsigned)p.B);
   return dispatch(p.dtype, p.N, [&](auto t, auto l) {
     using T = decltype(t);
     constexpr int LPC = decltype(l)::value;
+    if (geo.nseg > 1) {
+      Geo ga = geo;  // the first pass has smaller CTAs over the same segments
+      ga.nblk = (geo.Dg + NT / LPC - 1) / (NT / LPC);
+      scan_bwd_agg_kernel<T, LPC>
+          <<<dim3((unsigned)(ga.nblk * p.G), geo.nseg - 1, (unsigned)p.B), NT, 0, s>>>(p, ga, sc.seg);
+    }
     constexpr int bytes = (int)sizeof(BwdSmem<LPC>);
     auto kern = scan_bwd_kernel<T, LPC>;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return (int)MOGT_ERR_LAUNCH;
-    kern<<<grid, NTB, bytes, s>>>(p, geo, sc);
+    kern<<<dim3((unsigned)(geo.nblk * p.G), geo.nseg, (unsigned)p.B), NTB, bytes, s>>>(p, geo, sc);
     const int64_t nbc = p.B * p.L * p.G * 2 * p.N;
     if (nbc > 0) reduce_bc_kernel<T><<<(unsigned)((nbc + 255) / 256), 256, 0, s>>>(p, geo.nblk, NP, sc.bc);
     const int64_t np = p.D * p.N + 2 * p.D;
-    reduce_param_kernel<<<(unsigned)((np + 255) / 256), 256, 0, s>>>(p, NP, p.B, sc);
+    reduce_param_kernel<<<(unsigned)((np + 255) / 256), 256, 0, s>>>(p, NP, geo.nseg * p.B, sc);
     return mogt_host::launch_status();
   });
 }

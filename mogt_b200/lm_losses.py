@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .selective import _DTYPES, _cuda, _ptr, _stream
+from .selective import _CODE, _DTYPES, _cuda, _f32, _ptr
 
 __all__ = ["token_logprobs", "policy_loss", "preference_loss"]
 
@@ -36,7 +36,9 @@ def _rows(what, logits, labels, mask):
         raise ValueError(f"{what}: mask must be [B, L] bool")
     if logits.stride(2) != 1 and logits.shape[2] > 1:
         logits = logits.contiguous()
-    return logits, labels.to(torch.int64).contiguous(), None if mask is None else mask.contiguous()
+    if labels.dtype != torch.int64 or not labels.is_contiguous():
+        labels = labels.to(torch.int64).contiguous()
+    return logits, labels, None if mask is None else mask.contiguous()
 
 
 def _grad_like(logits):
@@ -54,23 +56,20 @@ def _logprob_fwd(logits, labels, mask, want_stats):
     dev = logits.device
     lp = torch.empty(B, L, dtype=torch.float32, device=dev)
     stats = torch.empty(B, L, 2, dtype=torch.float32, device=dev) if want_stats else None
-    with torch.cuda.device(dev):
-        N.check(N.lib().mogt_logprob_fwd(logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
-                                         _ptr(mask), B, L, V, N.dtype_code(logits.dtype), lp.data_ptr(), _ptr(stats),
-                                         _stream(dev)), "mogt_logprob_fwd")
+    N.launch("mogt_logprob_fwd", dev, logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
+             _ptr(mask), B, L, V, _CODE[logits.dtype], lp.data_ptr(), _ptr(stats))
     return lp, stats
 
 
 def _logprob_bwd(logits, labels, mask, stats, coef, coef_div, scale):
+    """stats, coef: addresses of f32 [B, L, 2] and [B * L / coef_div]."""
     B, L, V = logits.shape
     dev = logits.device
     d = _grad_like(logits)
-    scale = None if scale is None else scale.to(torch.float32).contiguous()
-    with torch.cuda.device(dev):
-        N.check(N.lib().mogt_logprob_bwd(logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
-                                         _ptr(mask), stats.data_ptr(), coef.data_ptr(), coef_div, _ptr(scale),
-                                         d.data_ptr(), d.stride(0), d.stride(1), B, L, V, N.dtype_code(logits.dtype),
-                                         _stream(dev)), "mogt_logprob_bwd")
+    scale = _f32(scale)
+    N.launch("mogt_logprob_bwd", dev, logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
+             _ptr(mask), stats, coef, coef_div, _ptr(scale), d.data_ptr(), d.stride(0), d.stride(1), B, L, V,
+             _CODE[logits.dtype])
     return d
 
 
@@ -85,7 +84,8 @@ class _TokenLogprobsFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         logits, labels, mask, stats = ctx.saved_tensors
-        return _logprob_bwd(logits, labels, mask, stats, g.to(torch.float32).contiguous(), 1, None), None, None
+        g = _f32(g)
+        return _logprob_bwd(logits, labels, mask, stats.data_ptr(), g.data_ptr(), 1, None), None, None
 
 
 def token_logprobs(logits, labels, *, mask=None):
@@ -100,26 +100,25 @@ def token_logprobs(logits, labels, *, mask=None):
 
 
 def _policy(logits, labels, mask, old, ref, adv, lo, hi, kl, want_grad):
+    """loss, lp, work, dlogits.  work (f32, n = B L) holds the rows' statistics
+    [n, 2] (with a gradient), the coefficients [n] and the kernels' scratch."""
     B, L, V = logits.shape
+    n = B * L
     dev = logits.device
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    lp, coef = (torch.empty(B, L, dtype=torch.float32, device=dev) for _ in range(2))
-    stats = d = None
-    if want_grad:
-        stats = torch.empty(B, L, 2, dtype=torch.float32, device=dev)
-        d = _grad_like(logits)
-    lib = N.lib()
-    nbytes = lib.mogt_policy_loss_scratch_bytes(B, L)
+    lp = torch.empty(B, L, dtype=torch.float32, device=dev)
+    nbytes = N.lib().mogt_policy_loss_scratch_bytes(B, L)
+    off = 2 * n if want_grad else 0
+    work = torch.empty(off + n + nbytes // 4, dtype=torch.float32, device=dev)
+    d = _grad_like(logits) if want_grad else None
     a_sb, a_sl = (adv.stride(0), 0) if adv.ndim == 1 else adv.stride()
-    with torch.cuda.device(dev):
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        N.check(lib.mogt_policy_loss(logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
-                                     _ptr(mask), old.data_ptr(), _ptr(ref), adv.data_ptr(), a_sb, a_sl, lo, hi, kl,
-                                     loss.data_ptr(), lp.data_ptr(), _ptr(stats), coef.data_ptr(), _ptr(d),
-                                     0 if d is None else d.stride(0), 0 if d is None else d.stride(1), B, L, V,
-                                     N.dtype_code(logits.dtype), scratch.data_ptr(), nbytes, _stream(dev)),
-                "mogt_policy_loss")
-    return loss, lp, stats, coef, d
+    d_sb, d_sl = (d.stride(0), d.stride(1)) if want_grad else (0, 0)
+    at = work.data_ptr()
+    N.launch("mogt_policy_loss", dev, logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
+             _ptr(mask), old.data_ptr(), _ptr(ref), adv.data_ptr(), a_sb, a_sl, lo, hi, kl, loss.data_ptr(),
+             lp.data_ptr(), at if want_grad else None, at + 4 * off, _ptr(d), d_sb, d_sl, B, L, V,
+             _CODE[logits.dtype], at + 4 * (off + n), nbytes)
+    return loss, lp, work, d
 
 
 class _PolicyLossFn(torch.autograd.Function):
@@ -131,9 +130,9 @@ class _PolicyLossFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, labels, mask, old, ref, adv, lo, hi, kl):
-        with torch.autograd.profiler.record_function("mogt.policy_loss.forward"):
-            loss, lp, stats, coef, d = _policy(logits, labels, mask, old, ref, adv, lo, hi, kl, True)
-        ctx.save_for_backward(logits, labels, mask, stats, coef)
+        with N.tag("mogt.policy_loss.forward"):
+            loss, lp, work, d = _policy(logits, labels, mask, old, ref, adv, lo, hi, kl, True)
+        ctx.save_for_backward(logits, labels, mask, work)
         ctx.grad = d
         ctx.mark_non_differentiable(lp)
         return loss, lp
@@ -142,23 +141,23 @@ class _PolicyLossFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _glp):
         d, ctx.grad = ctx.grad, None
-        with torch.autograd.profiler.record_function("mogt.policy_loss.backward"):
+        with N.tag("mogt.policy_loss.backward"):
             if d is None:
-                logits, labels, mask, stats, coef = ctx.saved_tensors
-                d = _logprob_bwd(logits, labels, mask, stats, coef, 1, g)
+                logits, labels, mask, work = ctx.saved_tensors
+                at = work.data_ptr()
+                d = _logprob_bwd(logits, labels, mask, at, at + 8 * labels.numel(), 1, g)
             else:
                 base = d if d.is_contiguous() else d._base
-                g = g.to(torch.float32).contiguous()
-                with torch.cuda.device(d.device):
-                    N.check(N.lib().mogt_scale_unless_one(base.data_ptr(), base.numel(), N.dtype_code(d.dtype),
-                                                          g.data_ptr(), _stream(d.device)), "mogt_scale_unless_one")
-        return (d,) + (None,) * 8
+                g = _f32(g)
+                N.launch("mogt_scale_unless_one", d.device, base.data_ptr(), base.numel(), _CODE[d.dtype],
+                         g.data_ptr())
+        return d, None, None, None, None, None, None, None, None
 
 
 def _token_f32(what, name, t, shape):
     if t.shape != shape:
         raise ValueError(f"{what}: {name} must be {list(shape)}")
-    return t.detach().to(torch.float32).contiguous()
+    return _f32(t.detach())
 
 
 def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, mask=None, clip_low=0.2, clip_high=0.2,
@@ -188,28 +187,29 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
         loss, lp = _PolicyLossFn.apply(logits, labels, mask, old, ref, adv, float(clip_low), float(clip_high),
                                        float(kl_coef))
     else:
-        with torch.autograd.profiler.record_function("mogt.policy_loss"):
+        with N.tag("mogt.policy_loss"):
             loss, lp = _policy(logits, labels, mask, old, ref, adv, float(clip_low), float(clip_high), float(kl_coef),
                                False)[:2]
     return (loss, lp) if return_logprobs else loss
 
 
 def _preference(logits, labels, mask, ref, beta, eps, want_grad):
+    """loss, seq, coef, stats."""
     B, L, _ = logits.shape
     dev = logits.device
     lp, stats = _logprob_fwd(logits, labels, mask, want_grad)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    seq, coef = (torch.empty(B, dtype=torch.float32, device=dev) for _ in range(2))
-    with torch.cuda.device(dev):
-        N.check(N.lib().mogt_preference_pairs(lp.data_ptr(), ref.data_ptr(), B // 2, L, beta, eps, loss.data_ptr(),
-                                              seq.data_ptr(), coef.data_ptr(), _stream(dev)), "mogt_preference_pairs")
+    seq = torch.empty(B, dtype=torch.float32, device=dev)
+    coef = torch.empty(B, dtype=torch.float32, device=dev)
+    N.launch("mogt_preference_pairs", dev, lp.data_ptr(), ref.data_ptr(), B // 2, L, beta, eps, loss.data_ptr(),
+             seq.data_ptr(), coef.data_ptr())
     return loss, seq, coef, stats
 
 
 class _PreferenceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, mask, ref, beta, eps):
-        with torch.autograd.profiler.record_function("mogt.preference_loss.forward"):
+        with N.tag("mogt.preference_loss.forward"):
             loss, seq, coef, stats = _preference(logits, labels, mask, ref, beta, eps, True)
         ctx.save_for_backward(logits, labels, mask, stats, coef)
         ctx.mark_non_differentiable(seq)
@@ -219,9 +219,9 @@ class _PreferenceLossFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _gseq):
         logits, labels, mask, stats, coef = ctx.saved_tensors
-        with torch.autograd.profiler.record_function("mogt.preference_loss.backward"):
-            d = _logprob_bwd(logits, labels, mask, stats, coef, max(logits.shape[1], 1), g)
-        return (d,) + (None,) * 5
+        with N.tag("mogt.preference_loss.backward"):
+            d = _logprob_bwd(logits, labels, mask, stats.data_ptr(), coef.data_ptr(), max(logits.shape[1], 1), g)
+        return d, None, None, None, None, None
 
 
 def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0.0, mask=None, return_logprobs=False):
@@ -245,6 +245,6 @@ def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0
     if torch.is_grad_enabled() and logits.requires_grad:
         loss, seq = _PreferenceLossFn.apply(logits, labels, mask, ref, float(beta), float(label_smoothing))
     else:
-        with torch.autograd.profiler.record_function("mogt.preference_loss"):
+        with N.tag("mogt.preference_loss"):
             loss, seq = _preference(logits, labels, mask, ref, float(beta), float(label_smoothing), False)[:2]
     return (loss, seq) if return_logprobs else loss

@@ -41,24 +41,29 @@ _MAX_STATES = 128
 def _cuda(what, *ts):
     dev = ts[0].device
     for t in ts:
-        if t is not None and t.device.type != "cuda":
+        if t is not None and not t.is_cuda:
             raise ValueError(f"{what} requires CUDA tensors")
         if t is not None and t.device != dev:
             raise ValueError(f"{what}: all tensors must be on one device")
     return dev
 
 
+_MAX_STRIDE = 1 << 27   # the scan's kernels step over a tile's tokens with 32-bit offsets
+
+
 def _dense_last(t):
-    """t itself when its last dimension is dense, else a contiguous copy."""
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t itself when its last dimension is dense (and its rows are not absurdly
+    far apart), else a contiguous copy."""
+    if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) <= _MAX_STRIDE):
+        return t
+    return t.contiguous()
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(dev):
-    return torch.cuda.current_stream(dev).cuda_stream
+_CODE = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
 
 
 def _lengths(lengths, B, what):
@@ -66,11 +71,13 @@ def _lengths(lengths, B, what):
         return None
     if lengths.shape != (B,) or lengths.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"{what}: lengths must be [B] int64 or int32")
-    return lengths.to(torch.int64).contiguous()
+    return lengths if lengths.dtype == torch.int64 and lengths.is_contiguous() else lengths.to(torch.int64).contiguous()
 
 
 def _f32(t):
-    return None if t is None else t.to(torch.float32).contiguous()
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.to(torch.float32).contiguous()
 
 
 def _activation(activation):
@@ -97,7 +104,7 @@ def _conv_params(weight, bias, D, what):
 class _CausalConvFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, initial_state, lengths, silu, return_state):
-        with torch.autograd.profiler.record_function("mogt.causal_conv.forward"):
+        with N.tag("mogt.causal_conv.forward"):
             y, fin = _conv_fwd(x, weight, bias, initial_state, lengths, silu, return_state)
         ctx.save_for_backward(x, weight, bias, initial_state, lengths)
         ctx.silu = silu
@@ -119,15 +126,13 @@ class _CausalConvFn(torch.autograd.Function):
         dinit = None
         if init is not None and ctx.needs_input_grad[3]:
             dinit = torch.empty(B, K - 1, D, dtype=x.dtype, device=dev)
-        lib = N.lib()
-        nbytes = lib.mogt_causal_conv_bwd_scratch_bytes(B, L, D, K)
-        with torch.autograd.profiler.record_function("mogt.causal_conv.backward"), torch.cuda.device(dev):
-            scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-            N.check(lib.mogt_causal_conv_bwd(
-                x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias), _ptr(init), _ptr(lengths),
-                dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dfinal), dx.data_ptr(), dw.data_ptr(), _ptr(db),
-                _ptr(dinit), B, L, D, K, ctx.silu, N.dtype_code(x.dtype), N.dtype_code(weight.dtype),
-                scratch.data_ptr(), scratch.numel(), _stream(dev)), "mogt_causal_conv_bwd")
+        nbytes = max(16, N.lib().mogt_causal_conv_bwd_scratch_bytes(B, L, D, K))
+        with N.tag("mogt.causal_conv.backward"):
+            scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            N.launch("mogt_causal_conv_bwd", dev, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias),
+                     _ptr(init), _ptr(lengths), dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dfinal), dx.data_ptr(),
+                     dw.data_ptr(), _ptr(db), _ptr(dinit), B, L, D, K, ctx.silu, _CODE[x.dtype], _CODE[weight.dtype],
+                     scratch.data_ptr(), nbytes)
         return dx, dw, db, dinit, None, None, None
 
 
@@ -137,11 +142,8 @@ def _conv_fwd(x, weight, bias, init, lengths, silu, return_state):
     dev = x.device
     y = torch.empty(B, L, D, dtype=x.dtype, device=dev)
     fin = torch.empty(B, K - 1, D, dtype=x.dtype, device=dev) if return_state else None
-    with torch.cuda.device(dev):
-        N.check(N.lib().mogt_causal_conv_fwd(
-            x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias), _ptr(init), _ptr(lengths),
-            y.data_ptr(), _ptr(fin), B, L, D, K, silu, N.dtype_code(x.dtype), N.dtype_code(weight.dtype),
-            _stream(dev)), "mogt_causal_conv_fwd")
+    N.launch("mogt_causal_conv_fwd", dev, x.data_ptr(), x.stride(0), x.stride(1), weight.data_ptr(), _ptr(bias),
+             _ptr(init), _ptr(lengths), y.data_ptr(), _ptr(fin), B, L, D, K, silu, _CODE[x.dtype], _CODE[weight.dtype])
     return y, fin
 
 
@@ -167,7 +169,7 @@ def causal_conv(x, weight, bias=None, *, activation="silu", initial_state=None, 
     x = _dense_last(x)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, initial_state)):
         return _CausalConvFn.apply(x, weight, bias, initial_state, lengths, silu, bool(return_state))
-    with torch.autograd.profiler.record_function("mogt.causal_conv"):
+    with N.tag("mogt.causal_conv"):
         y, fin = _conv_fwd(x, weight, bias, initial_state, lengths, silu, return_state)
     return (y, fin) if return_state else y
 
@@ -189,11 +191,8 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
             raise ValueError(f"{what}: state must be a contiguous [B, K-1, D] in x's dtype")
     x = _dense_last(x)
     y = torch.empty(B, D, dtype=x.dtype, device=dev)
-    with torch.cuda.device(dev):
-        N.check(N.lib().mogt_causal_conv_step(
-            x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _ptr(bias), y.data_ptr(),
-            new_state.data_ptr(), B, D, K, silu, N.dtype_code(x.dtype), N.dtype_code(weight.dtype), _stream(dev)),
-            "mogt_causal_conv_step")
+    N.launch("mogt_causal_conv_step", dev, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _ptr(bias),
+             y.data_ptr(), new_state.data_ptr(), B, D, K, silu, _CODE[x.dtype], _CODE[weight.dtype])
     return y
 
 
@@ -206,7 +205,9 @@ def _grouped(t, what, lead):
         t = t.unsqueeze(-2)
     if t.ndim != len(lead) + 2 or t.shape[:len(lead)] != lead:
         raise ValueError(f"{what}: B and C must be {list(lead)} + [N] or [G, N]")
-    return _dense_last(t)
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-3) <= _MAX_STRIDE:
+        return t
+    return t.contiguous()
 
 
 def _check_scan(what, u, delta, A, Bm, Cm, D, z, delta_bias):
@@ -246,7 +247,7 @@ def _scan_args(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus):
     a.A, a.Dskip, a.bias, a.init, a.lengths = A.data_ptr(), _ptr(D), _ptr(bias), _ptr(init), _ptr(lengths)
     a.B, a.L, a.D = u.shape
     a.N, a.G = A.shape[1], Bm.shape[2]
-    a.softplus, a.dtype = int(softplus), N.dtype_code(u.dtype)
+    a.softplus, a.dtype = int(softplus), _CODE[u.dtype]
     return a
 
 
@@ -265,8 +266,7 @@ def _scan_fwd(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus, return_s
     nbytes = lib.mogt_selective_fwd_scratch_bytes(B, L, ch, n, a.G)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     a.scratch, a.scratch_bytes = _ptr(scratch), nbytes
-    with torch.cuda.device(dev):
-        N.check(lib.mogt_selective_scan_fwd(ctypes.byref(a), _stream(dev)), "mogt_selective_scan_fwd")
+    N.launch("mogt_selective_scan_fwd", dev, ctypes.byref(a))
     return out, fin, saved
 
 
@@ -274,7 +274,7 @@ class _SelectiveScanFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus, return_state):
         f = tuple(_f32(t) for t in (A, D, bias, init))
-        with torch.autograd.profiler.record_function("mogt.selective_scan.forward"):
+        with N.tag("mogt.selective_scan.forward"):
             out, fin, saved = _scan_fwd(u, delta, f[0], Bm, Cm, f[1], z, f[2], f[3], lengths, softplus, return_state,
                                         True)
         ctx.save_for_backward(u, delta, A, Bm, Cm, D, z, bias, lengths, saved)
@@ -316,8 +316,8 @@ class _SelectiveScanFn(torch.autograd.Function):
         a.du, a.ddelta, a.dz, a.dB, a.dC = du.data_ptr(), ddelta.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
         a.dA, a.dD, a.dbias, a.dinit = dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dinit)
         a.scratch, a.scratch_bytes = scratch.data_ptr(), nbytes
-        with torch.autograd.profiler.record_function("mogt.selective_scan.backward"), torch.cuda.device(dev):
-            N.check(lib.mogt_selective_scan_bwd(ctypes.byref(a), _stream(dev)), "mogt_selective_scan_bwd")
+        with N.tag("mogt.selective_scan.backward"):
+            N.launch("mogt_selective_scan_bwd", dev, ctypes.byref(a))
         cast = lambda g, t: None if g is None else g.to(t.dtype)
         return (du, ddelta, cast(dA, A), dB, dC, cast(dD, D), dz, cast(dbias, bias),
                 None if dinit is None else dinit.to(ctx.init_dtype), None, None, None)
@@ -347,7 +347,7 @@ def selective_scan(u, delta, A, B, C, *, D=None, z=None, delta_bias=None, delta_
                                        for t in (u, delta, A, Bm, Cm, D, z, delta_bias, initial_state)):
         return _SelectiveScanFn.apply(u, delta, A, Bm, Cm, D, z, delta_bias, initial_state, lengths,
                                       bool(delta_softplus), bool(return_state))
-    with torch.autograd.profiler.record_function("mogt.selective_scan"):
+    with N.tag("mogt.selective_scan"):
         out, fin, _ = _scan_fwd(u, delta, _f32(A), Bm, Cm, _f32(D), z, _f32(delta_bias), _f32(initial_state), lengths,
                                 delta_softplus, return_state, False)
     return (out, fin) if return_state else out
@@ -372,10 +372,10 @@ def selective_scan_step(state, u, delta, A, B, C, *, D=None, z=None, delta_bias=
     u, delta, z = _dense_last(u), _dense_last(delta), _dense_last(z)
     A, D, delta_bias = _f32(A), _f32(D), _f32(delta_bias)
     y = torch.empty(bs, ch, dtype=u.dtype, device=dev)
-    with torch.cuda.device(dev):
-        N.check(N.lib().mogt_selective_step(
-            state.data_ptr(), new_state.data_ptr(), u.data_ptr(), u.stride(0), delta.data_ptr(), delta.stride(0),
-            _ptr(z), 0 if z is None else z.stride(0), Bm.data_ptr(), Bm.stride(0), Bm.stride(1), Cm.data_ptr(),
-            Cm.stride(0), Cm.stride(1), A.data_ptr(), _ptr(D), _ptr(delta_bias), y.data_ptr(), bs, ch, n, Bm.shape[1],
-            int(delta_softplus), N.dtype_code(u.dtype), _stream(dev)), "mogt_selective_step")
+    b_sb, b_sg, _ = Bm.stride()
+    c_sb, c_sg, _ = Cm.stride()
+    N.launch("mogt_selective_step", dev, state.data_ptr(), new_state.data_ptr(), u.data_ptr(), u.stride(0),
+             delta.data_ptr(), delta.stride(0), _ptr(z), 0 if z is None else z.stride(0), Bm.data_ptr(), b_sb, b_sg,
+             Cm.data_ptr(), c_sb, c_sg, A.data_ptr(), _ptr(D), _ptr(delta_bias), y.data_ptr(), bs, ch, n, Bm.shape[1],
+             int(delta_softplus), _CODE[u.dtype])
     return y
