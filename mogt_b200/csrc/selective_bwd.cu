@@ -76,10 +76,12 @@ __device__ __forceinline__ void put_copies(float4 (*dst)[LPC][Perm<LPC>::COPIES]
 
 template <int LPC>
 struct BwdSmem {
+  // two tiles: the one being worked on and the one being fetched
   float4 B[2][kTile][LPC][Perm<LPC>::COPIES], C[2][kTile][LPC][Perm<LPC>::COPIES];
-  float2 s1[NTB / 32][kTile][Lane<LPC>::CPW];   // (dt, x)
-  float4 s2[NTB / 32][kTile][Lane<LPC>::CPW];   // (dy, u, softplus', dout silu'(z))
-  float red[2][NTB / 32][kGroupB][2][Lane<LPC>::NP];
+  float2 s1[2][NTB / 32][kTile][Lane<LPC>::CPW];   // (dt, x)
+  float4 s2[2][NTB / 32][kTile][Lane<LPC>::CPW];   // (dy, u, softplus', dout silu'(z))
+  float4 hs[kTile / kGroupB - 1][NTB];             // states entering the tile's groups
+  float red[2][NTB / 32][kTile / 2][2][Lane<LPC>::NP];
 };
 
 // First pass over a split sequence: per segment (all but the first) the
@@ -271,86 +273,109 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
         if (gate) dz[(t + i) * p.D] = from_f32<T>(0.f);
       }
 
-  TileRaw<T, TPL, kGroupB> ru, rd, rz, ro;
+  // Fetching is spread over the groups of the tile before: a group's raw
+  // values are loaded when a group begins and staged when it ends, so few
+  // registers wait on memory.
+  GroupRaw<T, TPL> ru, rd, rz, ro;
   BcRaw<T, NP, NTB> rB, rC;
   float4 rs;
-  int last = 0;
-  auto fetch = [&](int64_t k) {
-    const int64_t t0 = k * kTile;
-    last = (int)min(len - 1 - t0, (int64_t)(kTile - 1));
-    rB.fetch(Bp + t0 * B_sl, B_sl, N, last);
-    rC.fetch(Cp + t0 * C_sl, C_sl, N, last);
-    rd.fetch(dp + t0 * d_sl, d_sl, tok, last);
-    ru.fetch(up + t0 * u_sl, u_sl, tok, last);
-    ro.fetch(op + t0 * o_sl, o_sl, tok, last);
-    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, tok, last);
-    rs = saved[k * p.D * LPC];
+  auto last_of = [&](int64_t k) { return (int)min(len - 1 - k * kTile, (int64_t)(kTile - 1)); };
+  auto fetch_bc = [&](int64_t k) {
+    rB.fetch(Bp + k * kTile * B_sl, B_sl, N, last_of(k));
+    rC.fetch(Cp + k * kTile * C_sl, C_sl, N, last_of(k));
   };
-  if (k0 < kl) fetch(kl - 1);
+  auto fetch = [&](int64_t k, int q) {
+    const int64_t t0 = k * kTile;
+    const int last = last_of(k), kk = q * kGroupB + tok;
+    rd.fetch(dp + t0 * d_sl, d_sl, kk, last);
+    ru.fetch(up + t0 * u_sl, u_sl, kk, last);
+    ro.fetch(op + t0 * o_sl, o_sl, kk, last);
+    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, kk, last);
+  };
+  auto stage = [&](int64_t k, int q) {
+    const int live = last_of(k);
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) {
+      const int kk = q * kGroupB + tok + i;
+      const float u = to_f32(ru.v[i]);
+      float dt = to_f32(rd.v[i]) + bias, dy = to_f32(ro.v[i]), ds = 1.f, zf = 0.f;
+      if (sp) {
+        const float e = exp_neg_abs(dt);
+        ds = __fdividef(dt >= 0.f ? 1.f : e, 1.f + e);
+        dt = softplus_e(dt, e);
+      }
+      if (gate) {
+        const float z = to_f32(rz.v[i]), sg = sigmoid(z);
+        zf = dy * sg * (1.f + z * (1.f - sg));
+        dy *= z * sg;
+      }
+      float x = dt * u;
+      // dead tokens, and lanes without a channel (they share the sums over channels)
+      if (kk > live || !w.ok) dt = x = dy = 0.f;
+      if (Q::DUP == 1 || w.owner()) {
+        sm.s1[k & 1][w.warp][kk][w.c] = make_float2(dt, x);
+        sm.s2[k & 1][w.warp][kk][w.c] = make_float4(dy, u, ds, zf);
+      }
+    }
+  };
+  if (k0 < kl) {
+    fetch_bc(kl - 1);
+    rs = saved[(kl - 1) * p.D * LPC];
+    put_copies<T, LPC, NTB>(sm.B[(kl - 1) & 1], rB, N, last_of(kl - 1));
+    put_copies<T, LPC, NTB>(sm.C[(kl - 1) & 1], rC, N, last_of(kl - 1));
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      fetch(kl - 1, q);
+      stage(kl - 1, q);
+    }
+    __syncthreads();
+  }
   for (int64_t k = kl - 1; k >= k0; --k) {
     const int64_t t0 = k * kTile;
-    const int buf = (int)(k & 1), live = last;
-    put_copies<T, LPC, NTB>(sm.B[buf], rB, N, live);
-    put_copies<T, LPC, NTB>(sm.C[buf], rC, N, live);
-#pragma unroll
-    for (int q = 0; q < NG; ++q)
-#pragma unroll
-      for (int i = 0; i < TPL; ++i) {
-        const int kk = q * kGroupB + tok + i;
-        const float u = to_f32(ru.v[q][i]);
-        float dt = to_f32(rd.v[q][i]) + bias, dy = to_f32(ro.v[q][i]), ds = 1.f, zf = 0.f;
-        if (sp) {
-          const float e = exp_neg_abs(dt);
-          ds = __fdividef(dt >= 0.f ? 1.f : e, 1.f + e);
-          dt = softplus_e(dt, e);
-        }
-        if (gate) {
-          const float z = to_f32(rz.v[q][i]), sg = sigmoid(z);
-          zf = dy * sg * (1.f + z * (1.f - sg));
-          dy *= z * sg;
-        }
-        float x = dt * u;
-        // dead tokens, and lanes without a channel (they share the sums over channels)
-        if (kk > live || !w.ok) dt = x = dy = 0.f;
-        if (Q::DUP == 1 || w.owner()) {
-          sm.s1[w.warp][kk][w.c] = make_float2(dt, x);
-          sm.s2[w.warp][kk][w.c] = make_float4(dy, u, ds, zf);
-        }
-      }
+    const int buf = (int)(k & 1), live = last_of(k);
+    const float2(*s1)[CPW] = sm.s1[buf][w.warp];
+    const float4(*s2)[CPW] = sm.s2[buf][w.warp];
     float4 h0 = Perm<LPC>::apply(rs, w.c);
     if (!w.ok) h0 = make_float4(0.f, 0.f, 0.f, 0.f);
-    __syncthreads();
-    if (k > k0) fetch(k - 1);
-    // states entering the tile's groups
-    F2 hs[NG][2];
-    hs[0][0] = f2(h0.x, h0.y);
-    hs[0][1] = f2(h0.z, h0.w);
+    // states entering the tile's groups: of the first and last in registers
+    F2 h01 = f2(h0.x, h0.y), h23 = f2(h0.z, h0.w);
+    const F2 hf01 = h01, hf23 = h23;
 #pragma unroll
     for (int q = 0; q + 1 < NG; ++q) {
-      F2 h01 = hs[q][0], h23 = hs[q][1];
+      if (q > 0) sm.hs[q - 1][threadIdx.x] = make_float4(un2(h01).x, un2(h01).y, un2(h23).x, un2(h23).y);
 #pragma unroll
       for (int i = 0; i < kGroupB; ++i) {
         const int kk = q * kGroupB + i;
-        const float2 s = sm.s1[w.warp][kk][w.c];
+        const float2 s = s1[kk][w.c];
         const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y);
         const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
         h01 = fma2(exp2_2(mul2(dt2, A01)), h01, mul2(x2, Bv.x));
         h23 = fma2(exp2_2(mul2(dt2, A23)), h23, mul2(x2, Bv.y));
       }
-      hs[q + 1][0] = h01;
-      hs[q + 1][1] = h23;
     }
     F2 tA01 = 0, tA23 = 0;
     float tD = 0.f, tb = 0.f;
     const int rows = (int)min(p.L - t0, (int64_t)kTile);
 #pragma unroll
     for (int q = NG - 1; q >= 0; --q) {
+      if (k > k0) {
+        fetch(k - 1, q);
+        if (q == NG - 1) fetch_bc(k - 1);
+        if (q == 0) rs = saved[(k - 1) * p.D * LPC];
+      }
+      if (q == 0) {
+        h01 = hf01;
+        h23 = hf23;
+      } else if (q < NG - 1) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.hs[q - 1][threadIdx.x]);
+        h01 = v.x;
+        h23 = v.y;
+      }
       F2 a[kGroupB][2], ph[kGroupB][2];
-      F2 h01 = hs[q][0], h23 = hs[q][1];
 #pragma unroll
       for (int i = 0; i < kGroupB; ++i) {
         const int kk = q * kGroupB + i;
-        const float2 s = sm.s1[w.warp][kk][w.c];
+        const float2 s = s1[kk][w.c];
         const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y);
         const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
         a[i][0] = exp2_2(mul2(dt2, A01));
@@ -364,8 +389,8 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
 #pragma unroll
       for (int i = kGroupB - 1; i >= 0; --i) {
         const int kk = q * kGroupB + i;
-        const float2 s = sm.s1[w.warp][kk][w.c];
-        const float dyv = sm.s2[w.warp][kk][w.c].x;
+        const float2 s = s1[kk][w.c];
+        const float dyv = s2[kk][w.c].x;
         const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y), dy2 = f2(dyv, dyv);
         const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
         const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(&sm.C[buf][kk][w.j][cq]);
@@ -380,22 +405,22 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
         tA23 = fma2(dt2, q23, tA23);
         cy01 = mul2(a[i][0], g01);
         cy23 = mul2(a[i][1], g23);
-        channel_sums<LPC>(mul2(g01, x2), mul2(g23, x2), mul2(dy2, h01), mul2(dy2, h23), sm.red[q & 1][w.warp][i], w.c,
-                          w.j);
+        channel_sums<LPC>(mul2(g01, x2), mul2(g23, x2), mul2(dy2, h01), mul2(dy2, h23),
+                          sm.red[kk / (kTile / 2)][w.warp][kk % (kTile / 2)], w.c, w.j);
       }
       sum_parts<LPC>(ysw, w.j);
 #pragma unroll
       for (int i = 0; i < TPL; ++i) {
         const int kk = q * kGroupB + i;  // + tok
-        const float dt = sm.s1[w.warp][kk + tok][w.c].x;
-        const float4 s2 = sm.s2[w.warp][kk + tok][w.c];  // (dy, u, softplus', dout silu'(z))
-        float gu = fmaf(dt, ysw[i][1], Dd * s2.x);
-        float gd = fmaf(s2.y, ysw[i][1], kLn2 * ysw[i][2]) * s2.z;
-        float gz = s2.w * fmaf(Dd, s2.y, ysw[i][0]);
+        const float dt = s1[kk + tok][w.c].x;
+        const float4 v = s2[kk + tok][w.c];  // (dy, u, softplus', dout silu'(z))
+        float gu = fmaf(dt, ysw[i][1], Dd * v.x);
+        float gd = fmaf(v.y, ysw[i][1], kLn2 * ysw[i][2]) * v.z;
+        float gz = v.w * fmaf(Dd, v.y, ysw[i][0]);
         if (kk + tok > live) {
           gu = gd = gz = 0.f;
         } else {
-          tD = fmaf(s2.x, s2.y, tD);
+          tD = fmaf(v.x, v.y, tD);
           tb += gd;
         }
         if (store && kk + tok < rows) {
@@ -405,16 +430,26 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
           if (gate) dz[o] = from_f32<T>(gz);
         }
       }
-      __syncthreads();
+      if (k > k0) {
+        stage(k - 1, q);
+        if (q == NG - 1) {
+          put_copies<T, LPC, NTB>(sm.B[buf ^ 1], rB, N, last_of(k - 1));
+          put_copies<T, LPC, NTB>(sm.C[buf ^ 1], rC, N, last_of(k - 1));
+        }
+      }
+      if (q % (NG / 2) == 0) {  // half a tile: add up the warps
+        const int half = q / (NG / 2);
+        __syncthreads();
 #pragma unroll
-      for (int i0 = 0; i0 < kGroupB * 2 * NP; i0 += NTB) {
-        const int i = i0 + threadIdx.x;
-        if (kGroupB * 2 * NP % NTB == 0 || i < kGroupB * 2 * NP) {
-          float v = 0.f;
+        for (int i0 = 0; i0 < kTile * NP; i0 += NTB) {
+          const int i = i0 + threadIdx.x;
+          if (kTile * NP % NTB == 0 || i < kTile * NP) {
+            float v = 0.f;
 #pragma unroll
-          for (int ww = 0; ww < NTB / 32; ++ww) v += (&sm.red[q & 1][ww][0][0][0])[i];
-          const int kk = q * kGroupB + i / (2 * NP);
-          if (kk <= live) bcp[(t0 + kk) * (2 * NP) + i % (2 * NP)] = v;
+            for (int ww = 0; ww < NTB / 32; ++ww) v += (&sm.red[half][ww][0][0][0])[i];
+            const int kk = half * (kTile / 2) + i / (2 * NP);
+            if (kk <= live) bcp[(t0 + kk) * (2 * NP) + i % (2 * NP)] = v;
+          }
         }
       }
     }

@@ -129,6 +129,16 @@ struct TileRaw {
   }
 };
 
+// The same for one group of a tile (first token kk of the lane).
+template <typename T, int TPL>
+struct GroupRaw {
+  T v[TPL];
+  __device__ __forceinline__ void fetch(const T* p, int sl, int kk, int last) {
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) v[i] = p[(int64_t)min(kk + i, last) * sl];
+  }
+};
+
 // A thread's share of one B or C tile (kTile x NP values over THREADS threads).
 template <typename T, int NP, int THREADS>
 struct BcRaw {
