@@ -32,9 +32,13 @@ namespace sel {
 #define MOGT_BWD_WARPS 16
 #endif
 #ifndef MOGT_BWD_CTAS
-#define MOGT_BWD_CTAS 2
+#define MOGT_BWD_CTAS 3
 #endif
-constexpr int kBwdWarps = MOGT_BWD_WARPS;  // warps per SM that the backward asks for
+// Segments of a backward: 3 CTAs fit on an SM; the first pass costs about a
+// quarter of the main one.
+inline int64_t bwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
+  return num_segments(B, L, D, N, G, NTB, 148 * MOGT_BWD_CTAS, 0.25f);
+}
 
 struct BwdScratch {
   SegScratch seg;
@@ -43,135 +47,162 @@ struct BwdScratch {
   float* dv;   // [nseg * B][2][D]: dD, dbias
 };
 
-// States in XORed order: slot i of a lane of channel c holds state i ^ (c & mask).
-template <int LPC>
-struct Perm {
-  static constexpr int COPIES = Lane<LPC>::CPW >= 4 ? 4 : Lane<LPC>::CPW;
-  static constexpr int MASK = COPIES - 1;
-  __device__ static __forceinline__ float4 apply(float4 v, int c) {
-    if (COPIES > 1 && (c & 1)) v = make_float4(v.y, v.x, v.w, v.z);
-    if (COPIES > 2 && (c & 2)) v = make_float4(v.z, v.w, v.x, v.y);
-    return v;
-  }
-};
-
-// One token's B or C: for every 4 states their COPIES orders side by side, so
-// that the lanes of a quarter warp (one part, 8 channels) read 64 consecutive
-// bytes: [part][copy][4].
-template <typename T, int LPC, int THREADS>
-__device__ __forceinline__ void put_copies(float4 (*dst)[LPC][Perm<LPC>::COPIES],
-                                           const BcRaw<T, Lane<LPC>::NP, THREADS>& r, int N, int last) {
+// One token's B or C: for every 4 states their COPIES orders
+// side by side, [part][copy][4], so that the lanes of one part read
+// neighbouring copies.
+template <typename T, int LPC>
+__device__ __forceinline__ void put_copies(float (*dst)[LPC][Perm<LPC>::COPIES][NS],
+                                           const BcRaw<T, Lane<LPC>::NP, NTB>& r, int N, int last) {
   constexpr int NP = Lane<LPC>::NP;
 #pragma unroll
-  for (int x = 0; x < BcRaw<T, NP, THREADS>::PER; ++x) {
-    const int i = threadIdx.x + x * THREADS;
-    if (kTile * NP % THREADS == 0 || i < kTile * NP) {
+  for (int x = 0; x < BcRaw<T, NP, NTB>::PER; ++x) {
+    const int i = threadIdx.x + x * NTB;
+    if (kTile * NP % NTB == 0 || i < kTile * NP) {
       const int k = i / NP, n = i % NP;
       const float v = r.get(x, N, last);
 #pragma unroll
-      for (int q = 0; q < Perm<LPC>::COPIES; ++q) reinterpret_cast<float*>(&dst[k][n / NS][q])[(n % NS) ^ q] = v;
+      for (int q = 0; q < Perm<LPC>::COPIES; ++q) dst[k][n / NS][q][(n % NS) ^ q] = v;
     }
+  }
+}
+
+// Tokens of a group of 4 that a lane takes: i-th of TPL.  The sums over parts
+// halve over neighbouring tokens first (they can start after two tokens).
+template <int LPC>
+__device__ __forceinline__ int group_token(int j, int i) {
+  if (LPC == 1) return i;
+  if (LPC == 2) return 2 * i + j;
+  const int t = j / (LPC >= 4 ? LPC / 4 : 1);
+  return (t >> 1) + 2 * (t & 1);
+}
+
+// Halving step over lane bit `bit` of the part number: lanes without the bit
+// keep (and receive the partner's share of) a, the others b.
+template <int LPC>
+__device__ __forceinline__ void halve(float (&a)[6], const float (&b)[6], int j, int bit) {
+  const bool hi = j & bit;
+#pragma unroll
+  for (int m = 0; m < 6; ++m) {
+    const float send = hi ? a[m] : b[m], keep = hi ? b[m] : a[m];
+    a[m] = keep + __shfl_xor_sync(0xffffffffu, send, bit * Lane<LPC>::CPW);
   }
 }
 
 template <int LPC>
 struct BwdSmem {
-  // two tiles: the one being worked on and the one being fetched
-  float4 B[2][kTile][LPC][Perm<LPC>::COPIES], C[2][kTile][LPC][Perm<LPC>::COPIES];
-  float2 s1[2][NTB / 32][kTile][Lane<LPC>::CPW];   // (dt, x)
-  float4 s2[2][NTB / 32][kTile][Lane<LPC>::CPW];   // (dy, u, softplus', dout silu'(z))
-  float4 hs[kTile / kGroupB - 1][NTB];             // states entering the tile's groups
+  float B[kTile][LPC][Perm<LPC>::COPIES][NS], C[kTile][LPC][Perm<LPC>::COPIES][NS];
+  // per token and channel pair; a group's slots take the next tile's values once the group is done
+  float4 s1[NTB / 32][kTile][Lane<LPC>::CPW];   // (dt, dt', x, x')
+  float4 s2[NTB / 32][kTile][Lane<LPC>::CPW];   // (dy, dy', u, u')
+  float4 s3[NTB / 32][kTile][Lane<LPC>::CPW];   // softplus' and dout silu'(z), both channels
+  float4 hs[kTile / kGroupB - 1][2][NTB];       // states entering the tile's groups but the last
+  float4 sumA[2][NTB];                          // a thread's sums for dA
   float red[2][NTB / 32][kTile / 2][2][Lane<LPC>::NP];
 };
 
 // First pass over a split sequence: per segment (all but the first) the
 // adjoint handed to the state before it, from nothing behind it, and sum dt.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(NT, LPC < 4 ? 3 : 4) scan_bwd_agg_kernel(const mogt_selective_args p,
+template <int LPC>
+struct AggSmem {
+  float C[2][kTile][Lane<LPC>::NP];
+  float4 stage[NT / 32][kTile][Lane<LPC>::CPW];  // (dt, dt', dy, dy')
+};
+
+template <typename T, int LPC, bool VEC>
+__global__ void __launch_bounds__(NT, LPC < 4 ? 2 : 4) scan_bwd_agg_kernel(const mogt_selective_args p,
                                                                          const Geo geo, const SegScratch seg) {
   using Q = Lane<LPC>;
-  constexpr int CPW = Q::CPW, TPL = Q::TPL, NP = Q::NP;
-  __shared__ __align__(16) float sC[2][kTile][NP];
-  __shared__ float2 stage[NT / 32][kTile][CPW];  // (dt, dy)
+  constexpr int TPL = Q::TPL, NP = Q::NP;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  AggSmem<LPC>& sm = *reinterpret_cast<AggSmem<LPC>*>(smem_raw);
   const Where<LPC> w(p, geo);
   const int64_t len = seq_len(p.lengths, w.b, p.L);
   const int64_t k0 = (int64_t)(blockIdx.y + 1) * geo.tps, k1 = min(k0 + geo.tps, geo.nck);
   const int64_t kl = min(k1, (len + kTile - 1) / kTile);
   const int64_t cell = w.b * p.D + w.d;
-  float A2[NS];
-  load_A<LPC>(A2, p, w);
-  const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
-  F2 g01 = 0, g23 = 0;
-  const float bias = p.bias ? p.bias[w.d] : 0.f;
-  const int tok = w.part_tok(), N = (int)p.N;
+  F2 A2[NS], g[NS];
+  const F2 l2e = f2(kLog2e, kLog2e);
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    A2[i] = mul2(w.state(p.A, w.d, p.N, w.j * NS + i), l2e);
+    g[i] = 0;
+  }
+  const float2 bias = w.param(p.bias);
+  const int tok = w.part_tok(), N = (int)p.N, one = w.ok1;
   const int d_sl = (int)p.delta_sl, z_sl = (int)p.z_sl, o_sl = (int)p.dout_sl, C_sl = (int)p.C_sl;
   const bool gate = p.z, sp = p.softplus;
   const T* dp = static_cast<const T*>(p.delta) + w.b * p.delta_sb + w.d;
   const T* zp = static_cast<const T*>(p.z) + w.b * p.z_sb + w.d;
   const T* op = static_cast<const T*>(p.dout) + w.b * p.dout_sb + w.d;
   const T* Cp = static_cast<const T*>(p.Cm) + w.b * p.C_sb + w.g * p.C_sg;
-  TileRaw<T, TPL, kGroup> rd, rz, ro;
+  Raws<T, TPL, kGroup, 2, VEC> rd, rz, ro;
   BcRaw<T, NP, NT> rC;
   int last = 0;
   auto fetch = [&](int64_t k) {
     const int64_t t0 = k * kTile;
     last = (int)min(len - 1 - t0, (int64_t)(kTile - 1));
     rC.fetch(Cp + t0 * C_sl, C_sl, N, last);
-    rd.fetch(dp + t0 * d_sl, d_sl, tok, last);
-    ro.fetch(op + t0 * o_sl, o_sl, tok, last);
-    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, tok, last);
+    rd.fetch(dp + t0 * d_sl, d_sl, tok, last, one);
+    ro.fetch(op + t0 * o_sl, o_sl, tok, last, one);
+    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, tok, last, one);
   };
-  float sdt = 0.f;
+  float2 sdt = make_float2(0.f, 0.f);
   if (k0 < kl) fetch(kl - 1);
   for (int64_t k = kl - 1; k >= k0; --k) {
     const int buf = (int)(k & 1), live = last;
-    rC.put(sC[buf], N, live);
+    rC.put(sm.C[buf], N, live);
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int i = 0; i < TPL; ++i) {
         const int kk = q * kGroup + tok + i;
-        float dt = to_f32(rd.v[q][i]) + bias, dy = to_f32(ro.v[q][i]);
-        if (sp) dt = softplus(dt);
+        float2 dy = ro.v[q][i].f();
         if (gate) {
-          const float z = to_f32(rz.v[q][i]);
-          dy *= z * sigmoid(z);
+          const float2 z = rz.v[q][i].f();
+          dy = make_float2(dy.x * z.x * sigmoid(z.x), dy.y * z.y * sigmoid(z.y));
         }
-        if (kk > live) dt = dy = 0.f;
-        if (Q::DUP == 1 || w.owner()) stage[w.warp][kk][w.c] = make_float2(dt, dy);
+        // x of make_dtx is not used here: dy takes its place
+        const DtX r = make_dtx(rd.v[q][i].f(), dy, bias, sp, kk > live);
+        if (kk > live) dy = make_float2(0.f, 0.f);
+        if (Q::DUP == 1 || w.owner()) sm.stage[w.warp][kk][w.c] = make_float4(r.dt.x, r.dt.y, dy.x, dy.y);
       }
     __syncthreads();
     if (k > k0) fetch(k - 1);
-    float sd = 0.f;
+    F2 sd = 0;
 #pragma unroll
     for (int kk = kTile - 1; kk >= 0; --kk) {
-      const float2 s = stage[w.warp][kk][w.c];
-      const F2 dt2 = f2(s.x, s.x), dy2 = f2(s.y, s.y);
-      const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(&sC[buf][kk][w.j * NS]);
-      g01 = mul2(exp2_2(mul2(dt2, A01)), fma2(Cv.x, dy2, g01));
-      g23 = mul2(exp2_2(mul2(dt2, A23)), fma2(Cv.y, dy2, g23));
-      sd += s.x;
+      const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&sm.stage[w.warp][kk][w.c]);
+      F2 Cn[NS];
+      twice4(Cn, &sm.C[buf][kk][w.j * NS]);
+#pragma unroll
+      for (int m = 0; m < NS; ++m) g[m] = mul2(exp2_2(mul2(s.x, A2[m])), fma2(Cn[m], s.y, g[m]));
+      sd = add2(sd, s.x);
     }
-    sdt += sd;
+    const float2 v = un2(sd);
+    sdt = make_float2(sdt.x + v.x, sdt.y + v.y);
     __syncwarp();
   }
-  if (w.ok) {
-    const float2 a = un2(g01), b = un2(g23);
-    const int64_t i = blockIdx.y * p.B * p.D + cell;
-    seg.loc[i * LPC + w.j] = make_float4(a.x, a.y, b.x, b.y);
-    if (w.j == 0) seg.sdt[i] = sdt;
+  const int64_t i = blockIdx.y * p.B * p.D + cell;
+  w.put4(seg.loc + w.j, i, g);
+  if (w.j == 0) {
+    if (w.ok) seg.sdt[i] = sdt.x;
+    if (w.ok1) seg.sdt[i + 1] = sdt.y;
   }
 }
 
-// Sums the 8 terms of one token (dB: v[0..3], dC: v[4..7], XORed order) over
-// the warp's channels and leaves them in row r[2][NP] of shared memory.
+// Sums the 8 terms of one token (dB: b, dC: c, XORed order) over the warp's
+// channels and leaves them in row r[2][NP] of shared memory.
 template <int LPC>
-__device__ __forceinline__ void channel_sums(F2 b01, F2 b23, F2 c01, F2 c23, float (*r)[Lane<LPC>::NP], int c,
+__device__ __forceinline__ void channel_sums(const F2 (&b)[NS], const F2 (&d)[NS], float (*r)[Lane<LPC>::NP], int c,
                                              int j) {
   constexpr int CPW = Lane<LPC>::CPW;
   constexpr unsigned ALL = 0xffffffffu;
-  const float2 b0 = un2(b01), b1 = un2(b23), c0 = un2(c01), c1 = un2(c23);
-  float v[8] = {b0.x, b0.y, b1.x, b1.y, c0.x, c0.y, c1.x, c1.y};
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    v[i] = hsum(b[i]);
+    v[NS + i] = hsum(d[i]);
+  }
   const int n0 = j * NS;
   if constexpr (CPW == 1) {
     *reinterpret_cast<float4*>(&r[0][n0]) = make_float4(v[0], v[1], v[2], v[3]);
@@ -203,8 +234,8 @@ __device__ __forceinline__ void channel_sums(F2 b01, F2 b23, F2 c01, F2 c23, flo
   }
 }
 
-template <typename T, int LPC>
-__global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
+template <typename T, int LPC, bool VEC>
+__global__ void __launch_bounds__(NTB, LPC == 4 ? MOGT_BWD_CTAS : (LPC == 1 ? 1 : 2))
     scan_bwd_kernel(const mogt_selective_args p, const Geo geo, const BwdScratch sc) {
   using Q = Lane<LPC, kGroupB>;
   constexpr int CPW = Q::CPW, TPL = Q::TPL, NP = Q::NP, NG = kTile / kGroupB;
@@ -217,37 +248,21 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
   const int64_t cell = w.b * p.D + w.d;
   const int cq = w.c & Perm<LPC>::MASK;
 
-  F2 A01, A23, cy01, cy23;
-  {
-    float A2[NS], cy[NS];
+  F2 A2[NS], cy[NS];
+  const F2 l2e = f2(kLog2e, kLog2e);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int n = w.j * NS + (i ^ cq);
-      A2[i] = (w.ok && n < p.N) ? p.A[w.d * p.N + n] * kLog2e : 0.f;
-      cy[i] = (p.dfinal && w.ok && n < p.N) ? p.dfinal[cell * p.N + n] : 0.f;
-    }
-#pragma unroll 4
-    for (int s = geo.nseg - 1; s > (int)blockIdx.y; --s) {
-      const int64_t i = (s - 1) * p.B * p.D + cell;
-      const float4 l = Perm<LPC>::apply(sc.seg.loc[i * LPC + w.j], w.c);
-      const float sd = sc.seg.sdt[i];
-      cy[0] = fmaf(fast_exp2(sd * A2[0]), cy[0], l.x);
-      cy[1] = fmaf(fast_exp2(sd * A2[1]), cy[1], l.y);
-      cy[2] = fmaf(fast_exp2(sd * A2[2]), cy[2], l.z);
-      cy[3] = fmaf(fast_exp2(sd * A2[3]), cy[3], l.w);
-    }
-    A01 = f2(A2[0], A2[1]);
-    A23 = f2(A2[2], A2[3]);
-    cy01 = f2(cy[0], cy[1]);
-    cy23 = f2(cy[2], cy[3]);
+  for (int i = 0; i < NS; ++i) {
+    const int n = w.j * NS + (i ^ cq);
+    A2[i] = mul2(w.state(p.A, w.d, p.N, n), l2e);
+    cy[i] = w.state(p.dfinal, cell, p.N, n);
   }
-  const F2 one = f2(1.f, 1.f);
-  F2 sumA01 = 0, sumA23 = 0;
-  float sumD = 0.f, sumb = 0.f;
-  const float Dd = p.Dskip ? p.Dskip[w.d] : 0.f;
-  const float bias = p.bias ? p.bias[w.d] : 0.f;
+  sm.sumA[0][threadIdx.x] = sm.sumA[1][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  chain<LPC, Where<LPC, kGroupB>, true>(cy, A2, sc.seg, geo.nseg - 2, -1, geo.nseg - 1 - (int)blockIdx.y, p.B * p.D,
+                                        cell, w);
+  float2 sumD = make_float2(0.f, 0.f), sumb = make_float2(0.f, 0.f);
+  const float2 Dd = w.param(p.Dskip), bias = w.param(p.bias);
   const bool gate = p.z, sp = p.softplus, store = w.ok && w.owner();
-  const int tok = w.part_tok(), N = (int)p.N, D = (int)p.D;
+  const int N = (int)p.N, D = (int)p.D, one = w.ok1;
   const int u_sl = (int)p.u_sl, d_sl = (int)p.delta_sl, z_sl = (int)p.z_sl, o_sl = (int)p.dout_sl,
             B_sl = (int)p.B_sl, C_sl = (int)p.C_sl;
   const T* up = static_cast<const T*>(p.u) + w.b * p.u_sb + w.d;
@@ -257,7 +272,7 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
   const T* Bp = static_cast<const T*>(p.Bm) + w.b * p.B_sb + w.g * p.B_sg;
   const T* Cp = static_cast<const T*>(p.Cm) + w.b * p.C_sb + w.g * p.C_sg;
   const float4* saved = reinterpret_cast<const float4*>(p.saved) + (w.b * geo.nck * p.D + w.d) * LPC + w.j;
-  const int64_t o0 = (w.b * p.L + tok) * p.D + w.d;
+  const int64_t o0 = w.b * p.L * p.D + w.d;
   T* du = static_cast<T*>(p.du) + o0;
   T* ddelta = static_cast<T*>(p.ddelta) + o0;
   T* dz = gate ? static_cast<T*>(p.dz) + o0 : nullptr;
@@ -266,176 +281,219 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
   // tiles behind the end
   for (int64_t t = max(kl, k0) * kTile; t < min(k1 * kTile, p.L); t += kGroupB)
 #pragma unroll
-    for (int i = 0; i < TPL; ++i)
-      if (store && t + tok + i < p.L) {
-        du[(t + i) * p.D] = from_f32<T>(0.f);
-        ddelta[(t + i) * p.D] = from_f32<T>(0.f);
-        if (gate) dz[(t + i) * p.D] = from_f32<T>(0.f);
+    for (int i = 0; i < TPL; ++i) {
+      const int64_t tt = t + group_token<LPC>(w.j, i);
+      if (store && tt < p.L) {
+        store_two<T, VEC>(du + tt * p.D, 0.f, 0.f, w.ok1);
+        store_two<T, VEC>(ddelta + tt * p.D, 0.f, 0.f, w.ok1);
+        if (gate) store_two<T, VEC>(dz + tt * p.D, 0.f, 0.f, w.ok1);
       }
+    }
 
   // Fetching is spread over the groups of the tile before: a group's raw
   // values are loaded when a group begins and staged when it ends, so few
   // registers wait on memory.
-  GroupRaw<T, TPL> ru, rd, rz, ro;
+  Two<T> ru[TPL], rd[TPL], rz[TPL], ro[TPL];
   BcRaw<T, NP, NTB> rB, rC;
-  float4 rs;
+  float4 rs0, rs1;
   auto last_of = [&](int64_t k) { return (int)min(len - 1 - k * kTile, (int64_t)(kTile - 1)); };
   auto fetch_bc = [&](int64_t k) {
     rB.fetch(Bp + k * kTile * B_sl, B_sl, N, last_of(k));
     rC.fetch(Cp + k * kTile * C_sl, C_sl, N, last_of(k));
   };
+  auto fetch_saved = [&](int64_t k) {
+    rs0 = saved[k * p.D * LPC];
+    rs1 = saved[(k * p.D + one) * LPC];
+  };
   auto fetch = [&](int64_t k, int q) {
     const int64_t t0 = k * kTile;
-    const int last = last_of(k), kk = q * kGroupB + tok;
-    rd.fetch(dp + t0 * d_sl, d_sl, kk, last);
-    ru.fetch(up + t0 * u_sl, u_sl, kk, last);
-    ro.fetch(op + t0 * o_sl, o_sl, kk, last);
-    if (gate) rz.fetch(zp + t0 * z_sl, z_sl, kk, last);
+    const int last = last_of(k);
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) {
+      const int64_t t = t0 + min(q * kGroupB + group_token<LPC>(w.j, i), last);
+      rd[i].template load<VEC>(dp + t * d_sl, one);
+      ru[i].template load<VEC>(up + t * u_sl, one);
+      ro[i].template load<VEC>(op + t * o_sl, one);
+      if (gate) rz[i].template load<VEC>(zp + t * z_sl, one);
+    }
   };
   auto stage = [&](int64_t k, int q) {
     const int live = last_of(k);
 #pragma unroll
     for (int i = 0; i < TPL; ++i) {
-      const int kk = q * kGroupB + tok + i;
-      const float u = to_f32(ru.v[i]);
-      float dt = to_f32(rd.v[i]) + bias, dy = to_f32(ro.v[i]), ds = 1.f, zf = 0.f;
-      if (sp) {
-        const float e = exp_neg_abs(dt);
-        ds = __fdividef(dt >= 0.f ? 1.f : e, 1.f + e);
-        dt = softplus_e(dt, e);
+      const int kk = q * kGroupB + group_token<LPC>(w.j, i);
+      const float2 uu = ru[i].f(), dd = rd[i].f(), oo = ro[i].f();
+      const float2 zz = gate ? rz[i].f() : make_float2(0.f, 0.f);
+      const bool dead0 = kk > live || !w.ok, dead1 = kk > live || !w.ok1;
+      float r[2][6];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float u = e ? uu.y : uu.x, z = e ? zz.y : zz.x;
+        float dt = (e ? dd.y + bias.y : dd.x + bias.x), dy = e ? oo.y : oo.x, ds = 1.f, zf = 0.f;
+        if (sp) {
+          const float x = exp_neg_abs(dt);
+          ds = __fdividef(dt >= 0.f ? 1.f : x, 1.f + x);
+          dt = softplus_e(dt, x);
+        }
+        if (gate) {
+          const float sg = sigmoid(z);
+          zf = dy * sg * (1.f + z * (1.f - sg));
+          dy *= z * sg;
+        }
+        // dead tokens, and channels that do not exist (they share the sums over channels)
+        const bool dead = e ? dead1 : dead0;
+        r[e][0] = dead ? 0.f : dt;
+        r[e][1] = dead ? 0.f : dt * u;
+        r[e][2] = dead ? 0.f : dy;
+        r[e][3] = u;
+        r[e][4] = ds;
+        r[e][5] = zf;
       }
-      if (gate) {
-        const float z = to_f32(rz.v[i]), sg = sigmoid(z);
-        zf = dy * sg * (1.f + z * (1.f - sg));
-        dy *= z * sg;
-      }
-      float x = dt * u;
-      // dead tokens, and lanes without a channel (they share the sums over channels)
-      if (kk > live || !w.ok) dt = x = dy = 0.f;
       if (Q::DUP == 1 || w.owner()) {
-        sm.s1[k & 1][w.warp][kk][w.c] = make_float2(dt, x);
-        sm.s2[k & 1][w.warp][kk][w.c] = make_float4(dy, u, ds, zf);
+        sm.s1[w.warp][kk][w.c] = make_float4(r[0][0], r[1][0], r[0][1], r[1][1]);
+        sm.s2[w.warp][kk][w.c] = make_float4(r[0][2], r[1][2], r[0][3], r[1][3]);
+        sm.s3[w.warp][kk][w.c] = make_float4(r[0][4], r[1][4], r[0][5], r[1][5]);
       }
     }
   };
   if (k0 < kl) {
     fetch_bc(kl - 1);
-    rs = saved[(kl - 1) * p.D * LPC];
-    put_copies<T, LPC, NTB>(sm.B[(kl - 1) & 1], rB, N, last_of(kl - 1));
-    put_copies<T, LPC, NTB>(sm.C[(kl - 1) & 1], rC, N, last_of(kl - 1));
-#pragma unroll
+    fetch_saved(kl - 1);
+    put_copies<T, LPC>(sm.B, rB, N, last_of(kl - 1));
+    put_copies<T, LPC>(sm.C, rC, N, last_of(kl - 1));
+#pragma unroll 1
     for (int q = 0; q < NG; ++q) {
       fetch(kl - 1, q);
       stage(kl - 1, q);
     }
     __syncthreads();
   }
+  const float4(*s1)[CPW] = sm.s1[w.warp];
+  const float4(*s2)[CPW] = sm.s2[w.warp];
   for (int64_t k = kl - 1; k >= k0; --k) {
     const int64_t t0 = k * kTile;
-    const int buf = (int)(k & 1), live = last_of(k);
-    const float2(*s1)[CPW] = sm.s1[buf][w.warp];
-    const float4(*s2)[CPW] = sm.s2[buf][w.warp];
-    float4 h0 = Perm<LPC>::apply(rs, w.c);
-    if (!w.ok) h0 = make_float4(0.f, 0.f, 0.f, 0.f);
-    // states entering the tile's groups: of the first and last in registers
-    F2 h01 = f2(h0.x, h0.y), h23 = f2(h0.z, h0.w);
-    const F2 hf01 = h01, hf23 = h23;
-#pragma unroll
+    const int live = last_of(k);
+    // states entering the tile's groups wait in shared memory
+    F2 h[NS];
+    {
+      const float4 a = Perm<LPC>::apply(rs0, w.c), b = Perm<LPC>::apply(rs1, w.c);
+      h[0] = f2(w.ok ? a.x : 0.f, w.ok1 ? b.x : 0.f);
+      h[1] = f2(w.ok ? a.y : 0.f, w.ok1 ? b.y : 0.f);
+      h[2] = f2(w.ok ? a.z : 0.f, w.ok1 ? b.z : 0.f);
+      h[3] = f2(w.ok ? a.w : 0.f, w.ok1 ? b.w : 0.f);
+    }
+#pragma unroll 1
     for (int q = 0; q + 1 < NG; ++q) {
-      if (q > 0) sm.hs[q - 1][threadIdx.x] = make_float4(un2(h01).x, un2(h01).y, un2(h23).x, un2(h23).y);
+      *reinterpret_cast<ulonglong2*>(&sm.hs[q][0][threadIdx.x]) = make_ulonglong2(h[0], h[1]);
+      *reinterpret_cast<ulonglong2*>(&sm.hs[q][1][threadIdx.x]) = make_ulonglong2(h[2], h[3]);
 #pragma unroll
       for (int i = 0; i < kGroupB; ++i) {
         const int kk = q * kGroupB + i;
-        const float2 s = s1[kk][w.c];
-        const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y);
-        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
-        h01 = fma2(exp2_2(mul2(dt2, A01)), h01, mul2(x2, Bv.x));
-        h23 = fma2(exp2_2(mul2(dt2, A23)), h23, mul2(x2, Bv.y));
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&s1[kk][w.c]);
+        F2 Bn[NS];
+        twice4(Bn, sm.B[kk][w.j][cq]);
+#pragma unroll
+        for (int m = 0; m < NS; ++m) h[m] = fma2(exp2_2(mul2(s.x, A2[m])), h[m], mul2(s.y, Bn[m]));
       }
     }
-    F2 tA01 = 0, tA23 = 0;
-    float tD = 0.f, tb = 0.f;
+    F2 tA[NS] = {0, 0, 0, 0};
+    float2 tD = make_float2(0.f, 0.f), tb = make_float2(0.f, 0.f);
     const int rows = (int)min(p.L - t0, (int64_t)kTile);
-#pragma unroll
+#pragma unroll 1
     for (int q = NG - 1; q >= 0; --q) {
       if (k > k0) {
         fetch(k - 1, q);
-        if (q == NG - 1) fetch_bc(k - 1);
-        if (q == 0) rs = saved[(k - 1) * p.D * LPC];
+        if (q == 0) {
+          fetch_bc(k - 1);
+          fetch_saved(k - 1);
+        }
       }
-      if (q == 0) {
-        h01 = hf01;
-        h23 = hf23;
-      } else if (q < NG - 1) {
-        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&sm.hs[q - 1][threadIdx.x]);
-        h01 = v.x;
-        h23 = v.y;
+      const int kq = q * kGroupB;
+      if (q < NG - 1) {
+        const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(&sm.hs[q][0][threadIdx.x]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&sm.hs[q][1][threadIdx.x]);
+        h[0] = a.x;
+        h[1] = a.y;
+        h[2] = b.x;
+        h[3] = b.y;
       }
-      F2 a[kGroupB][2], ph[kGroupB][2];
+      // hh[i]: the state before token i, hh[i + 1] the one after it
+      F2 a[kGroupB][NS], hh[kGroupB + 1][NS];
+#pragma unroll
+      for (int m = 0; m < NS; ++m) hh[0][m] = h[m];
 #pragma unroll
       for (int i = 0; i < kGroupB; ++i) {
-        const int kk = q * kGroupB + i;
-        const float2 s = s1[kk][w.c];
-        const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y);
-        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
-        a[i][0] = exp2_2(mul2(dt2, A01));
-        a[i][1] = exp2_2(mul2(dt2, A23));
-        ph[i][0] = mul2(a[i][0], h01);
-        ph[i][1] = mul2(a[i][1], h23);
-        h01 = fma2(x2, Bv.x, ph[i][0]);
-        h23 = fma2(x2, Bv.y, ph[i][1]);
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&s1[kq + i][w.c]);
+        F2 Bn[NS];
+        twice4(Bn, sm.B[kq + i][w.j][cq]);
+#pragma unroll
+        for (int m = 0; m < NS; ++m) {
+          a[i][m] = exp2_2(mul2(s.x, A2[m]));
+          hh[i + 1][m] = fma2(a[i][m], hh[i][m], mul2(s.y, Bn[m]));
+        }
       }
-      float ysw[kGroupB][3];
+      float ysw[kGroupB][6];  // y, sum g B, sum A q of the pair, per token
 #pragma unroll
       for (int i = kGroupB - 1; i >= 0; --i) {
-        const int kk = q * kGroupB + i;
-        const float2 s = s1[kk][w.c];
-        const float dyv = s2[kk][w.c].x;
-        const F2 dt2 = f2(s.x, s.x), x2 = f2(s.y, s.y), dy2 = f2(dyv, dyv);
-        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sm.B[buf][kk][w.j][cq]);
-        const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(&sm.C[buf][kk][w.j][cq]);
-        h01 = fma2(x2, Bv.x, ph[i][0]);
-        h23 = fma2(x2, Bv.y, ph[i][1]);
-        const F2 g01 = fma2(Cv.x, dy2, cy01), g23 = fma2(Cv.y, dy2, cy23);
-        const F2 q01 = mul2(g01, ph[i][0]), q23 = mul2(g23, ph[i][1]);
-        ysw[i][0] = hsum(fma2(Cv.y, h23, mul2(Cv.x, h01)));
-        ysw[i][1] = hsum(fma2(Bv.y, g23, mul2(Bv.x, g01)));
-        ysw[i][2] = hsum(fma2(A23, q23, mul2(A01, q01)));
-        tA01 = fma2(dt2, q01, tA01);
-        tA23 = fma2(dt2, q23, tA23);
-        cy01 = mul2(a[i][0], g01);
-        cy23 = mul2(a[i][1], g23);
-        channel_sums<LPC>(mul2(g01, x2), mul2(g23, x2), mul2(dy2, h01), mul2(dy2, h23),
-                          sm.red[kk / (kTile / 2)][w.warp][kk % (kTile / 2)], w.c, w.j);
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&s1[kq + i][w.c]);
+        const F2 dy = *reinterpret_cast<const F2*>(&s2[kq + i][w.c]);
+        F2 Bn[NS], Cn[NS];
+        twice4(Bn, sm.B[kq + i][w.j][cq]);
+        twice4(Cn, sm.C[kq + i][w.j][cq]);
+        F2 y = 0, ss = 0, ww = 0, db[NS], dc[NS];
+#pragma unroll
+        for (int m = 0; m < NS; ++m) {
+          const F2 g = fma2(Cn[m], dy, cy[m]);
+          cy[m] = mul2(a[i][m], g);
+          const F2 qq = mul2(cy[m], hh[i][m]);  // g a h
+          y = m ? fma2(Cn[m], hh[i + 1][m], y) : mul2(Cn[m], hh[i + 1][m]);
+          ss = m ? fma2(Bn[m], g, ss) : mul2(Bn[m], g);
+          ww = m ? fma2(A2[m], qq, ww) : mul2(A2[m], qq);
+          tA[m] = fma2(s.x, qq, tA[m]);
+          db[m] = mul2(g, s.y);
+          dc[m] = mul2(dy, hh[i + 1][m]);
+        }
+        const float2 y2 = un2(y), s2v = un2(ss), w2 = un2(ww);
+        ysw[i][0] = y2.x;
+        ysw[i][1] = y2.y;
+        ysw[i][2] = s2v.x;
+        ysw[i][3] = s2v.y;
+        ysw[i][4] = w2.x;
+        ysw[i][5] = w2.y;
+        channel_sums<LPC>(db, dc, sm.red[q / (NG / 2)][w.warp][(kq + i) % (kTile / 2)], w.c, w.j);
+        if (LPC >= 2 && i % 2 == 0) halve<LPC>(ysw[i], ysw[i + 1], w.j, LPC / 2);
       }
-      sum_parts<LPC>(ysw, w.j);
+      if (LPC >= 4) {
+        halve<LPC>(ysw[0], ysw[2], w.j, LPC / 4);
+#pragma unroll
+        for (int bit = LPC / 8; bit > 0; bit >>= 1)
+#pragma unroll
+          for (int m = 0; m < 6; ++m) ysw[0][m] += __shfl_xor_sync(0xffffffffu, ysw[0][m], bit * CPW);
+      }
 #pragma unroll
       for (int i = 0; i < TPL; ++i) {
-        const int kk = q * kGroupB + i;  // + tok
-        const float dt = s1[kk + tok][w.c].x;
-        const float4 v = s2[kk + tok][w.c];  // (dy, u, softplus', dout silu'(z))
-        float gu = fmaf(dt, ysw[i][1], Dd * v.x);
-        float gd = fmaf(v.y, ysw[i][1], kLn2 * ysw[i][2]) * v.z;
-        float gz = v.w * fmaf(Dd, v.y, ysw[i][0]);
-        if (kk + tok > live) {
-          gu = gd = gz = 0.f;
+        const int kk = kq + group_token<LPC>(w.j, i);
+        const float(&r)[6] = ysw[LPC == 2 ? 2 * i : i];
+        const float4 v1 = s1[kk][w.c], v2 = s2[kk][w.c], v3 = sm.s3[w.warp][kk][w.c];
+        float u0 = fmaf(v1.x, r[2], Dd.x * v2.x), u1 = fmaf(v1.y, r[3], Dd.y * v2.y);
+        float d0 = fmaf(v2.z, r[2], kLn2 * r[4]) * v3.x, d1 = fmaf(v2.w, r[3], kLn2 * r[5]) * v3.y;
+        float z0 = v3.z * fmaf(Dd.x, v2.z, r[0]), z1 = v3.w * fmaf(Dd.y, v2.w, r[1]);
+        if (kk > live) {
+          u0 = u1 = d0 = d1 = z0 = z1 = 0.f;
         } else {
-          tD = fmaf(v.x, v.y, tD);
-          tb += gd;
+          tD = make_float2(fmaf(v2.x, v2.z, tD.x), fmaf(v2.y, v2.w, tD.y));
+          tb = make_float2(tb.x + d0, tb.y + d1);
         }
-        if (store && kk + tok < rows) {
+        if (store && kk < rows) {
           const int64_t o = (t0 + kk) * D;
-          du[o] = from_f32<T>(gu);
-          ddelta[o] = from_f32<T>(gd);
-          if (gate) dz[o] = from_f32<T>(gz);
+          store_two<T, VEC>(du + o, u0, u1, w.ok1);
+          store_two<T, VEC>(ddelta + o, d0, d1, w.ok1);
+          if (gate) store_two<T, VEC>(dz + o, z0, z1, w.ok1);
         }
       }
       if (k > k0) {
+        __syncwarp();  // the group's slots are free
         stage(k - 1, q);
-        if (q == NG - 1) {
-          put_copies<T, LPC, NTB>(sm.B[buf ^ 1], rB, N, last_of(k - 1));
-          put_copies<T, LPC, NTB>(sm.C[buf ^ 1], rC, N, last_of(k - 1));
-        }
       }
       if (q % (NG / 2) == 0) {  // half a tile: add up the warps
         const int half = q / (NG / 2);
@@ -453,31 +511,45 @@ __global__ void __launch_bounds__(NTB, LPC == 4 || LPC == 8 ? MOGT_BWD_CTAS : 1)
         }
       }
     }
-    sumA01 = fma2(one, tA01, sumA01);
-    sumA23 = fma2(one, tA23, sumA23);
-    sumD += tD;
-    sumb += tb;
-  }
-  if (!w.owner()) sumD = sumb = 0.f;
-  const int64_t row = blockIdx.y * p.B + w.b;
-  if (w.ok) {
-    const float2 a0 = un2(sumA01), a1 = un2(sumA23), c0 = un2(cy01), c1 = un2(cy23);
-    const float sa[NS] = {a0.x, a0.y, a1.x, a1.y}, cc[NS] = {c0.x, c0.y, c1.x, c1.y};
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int n = w.j * NS + (i ^ cq);
-      sc.dA[(row * p.D + w.d) * NP + n] = sa[i];
-      if (p.dinit && blockIdx.y == 0 && n < p.N) p.dinit[cell * p.N + n] = cc[i];
+    if (k > k0) {  // every warp is past its last use of this tile's B and C
+      put_copies<T, LPC>(sm.B, rB, N, last_of(k - 1));
+      put_copies<T, LPC>(sm.C, rC, N, last_of(k - 1));
+      __syncthreads();
     }
+    // tiles' sums first, then their sum: keeps the error of a long sequence small
+#pragma unroll
+    for (int m = 0; m < NS; m += 2) {
+      ulonglong2* v = reinterpret_cast<ulonglong2*>(&sm.sumA[m / 2][threadIdx.x]);
+      *v = make_ulonglong2(add2(v->x, tA[m]), add2(v->y, tA[m + 1]));
+    }
+    sumD = make_float2(sumD.x + tD.x, sumD.y + tD.y);
+    sumb = make_float2(sumb.x + tb.x, sumb.y + tb.y);
+  }
+  if (!w.owner()) sumD = sumb = make_float2(0.f, 0.f);
+  const int64_t row = blockIdx.y * p.B + w.b;
+#pragma unroll
+  for (int i = 0; i < NS; ++i) {
+    const int n = w.j * NS + (i ^ cq);
+    w.put_state(sc.dA, row * p.D + w.d, NP, n, reinterpret_cast<const F2*>(&sm.sumA[i / 2][threadIdx.x])[i % 2]);
+    if (p.dinit && blockIdx.y == 0) w.put_state(p.dinit, cell, p.N, n, cy[i]);
   }
 #pragma unroll
   for (int o = CPW; o < 32; o <<= 1) {
-    sumD += __shfl_xor_sync(0xffffffffu, sumD, o);
-    sumb += __shfl_xor_sync(0xffffffffu, sumb, o);
+    sumD.x += __shfl_xor_sync(0xffffffffu, sumD.x, o);
+    sumD.y += __shfl_xor_sync(0xffffffffu, sumD.y, o);
+    sumb.x += __shfl_xor_sync(0xffffffffu, sumb.x, o);
+    sumb.y += __shfl_xor_sync(0xffffffffu, sumb.y, o);
   }
-  if (w.ok && w.j == 0) {
-    sc.dv[(row * 2 + 0) * p.D + w.d] = sumD;
-    sc.dv[(row * 2 + 1) * p.D + w.d] = sumb;
+  if (w.j == 0) {
+    float* v = sc.dv + row * 2 * p.D + w.d;
+    if (w.ok) {
+      v[0] = sumD.x;
+      v[p.D] = sumb.x;
+    }
+    if (w.ok1) {
+      v[1] = sumD.y;
+      v[p.D + 1] = sumb.y;
+    }
   }
 }
 
@@ -520,7 +592,7 @@ __global__ void __launch_bounds__(256) reduce_param_kernel(const mogt_selective_
 }
 
 inline size_t bwd_floats(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G, int64_t nseg) {
-  const int64_t np = lpc_of(N) * NS, cpb = NTB / lpc_of(N);
+  const int64_t np = lpc_of(N) * NS, cpb = channels_per_cta(NTB, lpc_of(N));
   const int64_t seg = (int64_t)(seg_scratch_bytes(B, D, N, nseg) / sizeof(float) + 3) / 4 * 4;
   return (size_t)(seg + (D / G + cpb - 1) / cpb * B * G * L * 2 * np + nseg * B * D * (np + 2));
 }
@@ -533,7 +605,7 @@ using namespace mogt::sel;
 
 extern "C" size_t mogt_selective_bwd_scratch_bytes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
   if (B <= 0 || L < 0 || D <= 0 || N <= 0 || N > kMaxN || G <= 0 || D % G) return 0;
-  return bwd_floats(B, L, D, N, G, num_segments(B, L, D, N, G, NTB, kBwdWarps)) * sizeof(float);
+  return bwd_floats(B, L, D, N, G, bwd_segments(B, L, D, N, G)) * sizeof(float);
 }
 
 extern "C" int mogt_selective_scan_bwd(const mogt_selective_args* args, void* stream) {
@@ -548,7 +620,7 @@ extern "C" int mogt_selective_scan_bwd(const mogt_selective_args* args, void* st
   if (!p.scratch || p.scratch_bytes < mogt_selective_bwd_scratch_bytes(p.B, p.L, p.D, p.N, p.G))
     return MOGT_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(p.scratch) | reinterpret_cast<uintptr_t>(p.saved)) & 15u) return MOGT_ERR_ALIGN;
-  const Geo geo = geometry(p, NTB, kBwdWarps);
+  const Geo geo = geometry(p, NTB, bwd_segments(p.B, p.L, p.D, p.N, p.G));
   const int NP = lpc_of(p.N) * NS;
   BwdScratch sc;
   sc.seg = seg_scratch(p.scratch, p.B, p.D, p.N, geo.nseg);
@@ -556,20 +628,26 @@ extern "C" int mogt_selective_scan_bwd(const mogt_selective_args* args, void* st
   sc.dv = sc.dA + geo.nseg * p.B * p.D * NP;
   sc.bc = sc.dv + geo.nseg * p.B * 2 * p.D;
   cudaStream_t s = (cudaStream_t)stream;
+  const bool vec = pairs_aligned(p, true);
+  static_assert(NT == NTB, "the first pass takes the main pass's channel blocks");
   return dispatch(p.dtype, p.N, [&](auto t, auto l) {
     using T = decltype(t);
     constexpr int LPC = decltype(l)::value;
-    if (geo.nseg > 1) {
-      Geo ga = geo;  // the first pass has smaller CTAs over the same segments
-      ga.nblk = (geo.Dg + NT / LPC - 1) / (NT / LPC);
-      scan_bwd_agg_kernel<T, LPC>
-          <<<dim3((unsigned)(ga.nblk * p.G), geo.nseg - 1, (unsigned)p.B), NT, 0, s>>>(p, ga, sc.seg);
-    }
+    auto go = [&](auto kern, int bytes, int nseg, const auto& scratch) {
+      if (bytes > 48 * 1024 &&
+          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        return false;
+      kern<<<dim3((unsigned)(geo.nblk * p.G), nseg, (unsigned)p.B), NTB, bytes, s>>>(p, geo, scratch);
+      return true;
+    };
+    bool ok = true;
+    if (geo.nseg > 1)
+      ok = vec ? go(scan_bwd_agg_kernel<T, LPC, true>, (int)sizeof(AggSmem<LPC>), geo.nseg - 1, sc.seg)
+               : go(scan_bwd_agg_kernel<T, LPC, false>, (int)sizeof(AggSmem<LPC>), geo.nseg - 1, sc.seg);
     constexpr int bytes = (int)sizeof(BwdSmem<LPC>);
-    auto kern = scan_bwd_kernel<T, LPC>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-      return (int)MOGT_ERR_LAUNCH;
-    kern<<<dim3((unsigned)(geo.nblk * p.G), geo.nseg, (unsigned)p.B), NTB, bytes, s>>>(p, geo, sc);
+    ok = ok && (vec ? go(scan_bwd_kernel<T, LPC, true>, bytes, geo.nseg, sc)
+                    : go(scan_bwd_kernel<T, LPC, false>, bytes, geo.nseg, sc));
+    if (!ok) return (int)MOGT_ERR_LAUNCH;
     const int64_t nbc = p.B * p.L * p.G * 2 * p.N;
     if (nbc > 0) reduce_bc_kernel<T><<<(unsigned)((nbc + 255) / 256), 256, 0, s>>>(p, geo.nblk, NP, sc.bc);
     const int64_t np = p.D * p.N + 2 * p.D;

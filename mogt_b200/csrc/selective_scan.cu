@@ -6,68 +6,62 @@
 // 8 bytes per (token, channel) in bf16: at N = 16 the exponentials (16 a clock
 // and SM) bound it, not HBM.
 //
-// A thread keeps NS = 4 states of one channel in registers; LPC = N / 4
-// (rounded up to a power of two) lanes share a channel, so a warp holds
-// 32 / LPC channels.  Lane = channel + CPW * part.  Tokens come in groups of
-// 8: the LPC lanes of a channel split the group's tokens for what is done once
-// per (token, channel) (softplus, gate, loads, stores), hand (dt, dt u) to one
-// another through shared memory, and sum y over the parts with a butterfly
-// that leaves each lane the tokens it loaded.
+// A thread keeps NS = 4 states of two neighbouring channels in registers, the
+// pair in the halves of packed fp32 instructions; LPC = N / 4 (rounded up to a
+// power of two) lanes share a pair.  Lane = pair + CPW * part.  Tokens come in
+// tiles of 16 (the next tile's operands are loaded while one is worked on) and
+// groups of 8: the LPC lanes of a pair split a group's tokens for what is done
+// once per (token, channel) (softplus, gate, loads, stores), hand (dt, dt u)
+// to one another through shared memory, and sum y over the parts with a
+// butterfly that leaves each lane the tokens it loaded.
+//
+// When channels and sequences do not fill the GPU, a sequence is split into
+// segments: a first pass leaves each segment's state from zero and its sum of
+// dt, and a segment starts from the chain over those before it.
 #include "selective_scan.cuh"
 
 namespace mogt {
 namespace sel {
 
-#ifndef MOGT_FWD_WARPS
-#define MOGT_FWD_WARPS 16
-#endif
-#ifndef MOGT_FWD_CTAS
-#define MOGT_FWD_CTAS 4
-#endif
-constexpr int kFwdWarps = MOGT_FWD_WARPS;  // warps per SM that the forward asks for
+// Segments of a forward: 4 CTAs fit on an SM; the first pass costs about 0.7
+// of the main one (310 against 430 us at 32768 x 1536, N = 16).
+inline int64_t fwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
+  return num_segments(B, L, D, N, G, NT, 148 * 4, 0.7f);
+}
+
+template <int LPC, bool AGG>
+struct FwdSmem {
+  float B[2][kTile][Lane<LPC>::NP];
+  float4 stage[NT / 32][kTile][Lane<LPC>::CPW];  // (dt, dt', x, x')
+  float C[AGG ? 1 : 2][AGG ? 1 : kTile][Lane<LPC>::NP];
+};
 
 // grid = (channel blocks, segments, B).  AGG: the first pass over a split
 // sequence, which leaves each segment's state from zero and its sum of dt.
-template <typename T, int LPC, bool AGG>
-__global__ void __launch_bounds__(NT, LPC < 4 ? 3 : MOGT_FWD_CTAS) scan_fwd_kernel(const mogt_selective_args p, const Geo geo,
-                                                                     const SegScratch seg) {
+template <typename T, int LPC, bool VEC, bool AGG>
+__global__ void __launch_bounds__(NT, LPC < 4 ? 2 : 4) scan_fwd_kernel(const mogt_selective_args p, const Geo geo,
+                                                                       const SegScratch seg) {
   using Q = Lane<LPC>;
-  constexpr int CPW = Q::CPW, TPL = Q::TPL, NP = Q::NP;
-  __shared__ __align__(16) float sB[2][kTile][NP], sC[AGG ? 1 : 2][AGG ? 1 : kTile][NP];
-  __shared__ float2 stage[NT / 32][kTile][CPW];  // (dt, x)
+  constexpr int TPL = Q::TPL, NP = Q::NP;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  FwdSmem<LPC, AGG>& sm = *reinterpret_cast<FwdSmem<LPC, AGG>*>(smem_raw);
   const Where<LPC> w(p, geo);
   const int64_t len = seq_len(p.lengths, w.b, p.L);
   const int64_t k0 = (int64_t)blockIdx.y * geo.tps, k1 = min(k0 + geo.tps, geo.nck);
   const int64_t kl = min(k1, (len + kTile - 1) / kTile);  // first tile without a live token
   const int64_t cell = w.b * p.D + w.d;
 
-  float A2[NS];
-  load_A<LPC>(A2, p, w);
-  const F2 A01 = f2(A2[0], A2[1]), A23 = f2(A2[2], A2[3]);
-  F2 h01 = 0, h23 = 0;
-  if (!AGG) {
-    float h[NS];
+  F2 A2[NS], h[NS];
+  const F2 l2e = f2(kLog2e, kLog2e);
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      const int n = w.j * NS + i;
-      h[i] = (p.init && w.ok && n < p.N) ? p.init[cell * p.N + n] : 0.f;
-    }
-#pragma unroll 4
-    for (int s = 0; s < (int)blockIdx.y; ++s) {
-      const float4 l = seg.loc[(s * p.B * p.D + cell) * LPC + w.j];
-      const float sd = seg.sdt[s * p.B * p.D + cell];
-      h[0] = fmaf(fast_exp2(sd * A2[0]), h[0], l.x);
-      h[1] = fmaf(fast_exp2(sd * A2[1]), h[1], l.y);
-      h[2] = fmaf(fast_exp2(sd * A2[2]), h[2], l.z);
-      h[3] = fmaf(fast_exp2(sd * A2[3]), h[3], l.w);
-    }
-    h01 = f2(h[0], h[1]);
-    h23 = f2(h[2], h[3]);
+  for (int i = 0; i < NS; ++i) {
+    A2[i] = mul2(w.state(p.A, w.d, p.N, w.j * NS + i), l2e);
+    h[i] = AGG ? 0 : w.state(p.init, cell, p.N, w.j * NS + i);
   }
-  const float Dd = !AGG && p.Dskip ? p.Dskip[w.d] : 0.f;
-  const float bias = p.bias ? p.bias[w.d] : 0.f;
+  if (!AGG) chain<LPC, Where<LPC>, false>(h, A2, seg, 0, 1, blockIdx.y, p.B * p.D, cell, w);
+  const float2 Dd = AGG ? make_float2(0.f, 0.f) : w.param(p.Dskip), bias = w.param(p.bias);
   const bool gate = !AGG && p.z, sp = p.softplus, store = w.ok && w.owner();
-  const int tok = w.part_tok(), N = (int)p.N, D = (int)p.D;
+  const int tok = w.part_tok(), N = (int)p.N, D = (int)p.D, one = w.ok1;
   const int u_sl = (int)p.u_sl, d_sl = (int)p.delta_sl, z_sl = (int)p.z_sl, B_sl = (int)p.B_sl, C_sl = (int)p.C_sl;
   const T* up = static_cast<const T*>(p.u) + w.b * p.u_sb + k0 * kTile * p.u_sl + w.d;
   const T* dp = static_cast<const T*>(p.delta) + w.b * p.delta_sb + k0 * kTile * p.delta_sl + w.d;
@@ -75,27 +69,27 @@ __global__ void __launch_bounds__(NT, LPC < 4 ? 3 : MOGT_FWD_CTAS) scan_fwd_kern
   const T* Bp = static_cast<const T*>(p.Bm) + w.b * p.B_sb + w.g * p.B_sg + k0 * kTile * p.B_sl;
   const T* Cp = static_cast<const T*>(p.Cm) + w.b * p.C_sb + w.g * p.C_sg + k0 * kTile * p.C_sl;
   T* out = static_cast<T*>(p.out) + (w.b * p.L + k0 * kTile) * p.D + w.d;
-  float4* saved = AGG || !p.saved || !w.ok
+  float4* saved = AGG || !p.saved
                       ? nullptr
                       : reinterpret_cast<float4*>(p.saved) + ((w.b * geo.nck + k0) * p.D + w.d) * LPC + w.j;
 
-  TileRaw<T, TPL, kGroup> ru, rd, rz;
+  Raws<T, TPL, kGroup, 2, VEC> ru, rd, rz;
   BcRaw<T, NP, NT> rB, rC;
-  float sdt = 0.f;
+  float2 sdt = make_float2(0.f, 0.f);
   int last = 0;  // last live token of the fetched tile
   auto fetch = [&](int64_t k) {
     last = (int)min(len - 1 - k * kTile, (int64_t)(kTile - 1));
     rB.fetch(Bp, B_sl, N, last);
     Bp += (int64_t)kTile * B_sl;
-    rd.fetch(dp, d_sl, tok, last);
+    rd.fetch(dp, d_sl, tok, last, one);
     dp += (int64_t)kTile * d_sl;
-    ru.fetch(up, u_sl, tok, last);
+    ru.fetch(up, u_sl, tok, last, one);
     up += (int64_t)kTile * u_sl;
     if (!AGG) {
       rC.fetch(Cp, C_sl, N, last);
       Cp += (int64_t)kTile * C_sl;
       if (gate) {
-        rz.fetch(zp, z_sl, tok, last);
+        rz.fetch(zp, z_sl, tok, last, one);
         zp += (int64_t)kTile * z_sl;
       }
     }
@@ -104,48 +98,47 @@ __global__ void __launch_bounds__(NT, LPC < 4 ? 3 : MOGT_FWD_CTAS) scan_fwd_kern
   for (int64_t k = k0; k < kl; ++k) {
     const int buf = (int)(k & 1), live = last;
     if (saved) {
-      const float2 a = un2(h01), b = un2(h23);
-      *saved = make_float4(a.x, a.y, b.x, b.y);
+      w.put4(saved, 0, h);
       saved += (int64_t)D * LPC;
     }
-    rB.put(sB[buf], N, live);
-    if (!AGG) rC.put(sC[buf], N, live);
-    float u[2][TPL], gz[2][TPL];
+    rB.put(sm.B[buf], N, live);
+    if (!AGG) rC.put(sm.C[AGG ? 0 : buf], N, live);
+    float2 u[2][TPL], gz[2][TPL];
 #pragma unroll
     for (int q = 0; q < 2; ++q)
 #pragma unroll
       for (int i = 0; i < TPL; ++i) {
         const int kk = q * kGroup + tok + i;
-        u[q][i] = to_f32(ru.v[q][i]);
-        float dt = to_f32(rd.v[q][i]) + bias;
-        if (sp) dt = softplus(dt);
-        float x = dt * u[q][i];
-        if (kk > live) dt = x = 0.f;
-        if (Q::DUP == 1 || w.owner()) stage[w.warp][kk][w.c] = make_float2(dt, x);
+        u[q][i] = ru.v[q][i].f();
+        const DtX r = make_dtx(rd.v[q][i].f(), u[q][i], bias, sp, kk > live);
+        if (Q::DUP == 1 || w.owner()) sm.stage[w.warp][kk][w.c] = make_float4(r.dt.x, r.dt.y, r.x.x, r.x.y);
         if (gate) {
-          const float z = to_f32(rz.v[q][i]);
-          gz[q][i] = z * sigmoid(z);
+          const float2 z = rz.v[q][i].f();
+          gz[q][i] = make_float2(z.x * sigmoid(z.x), z.y * sigmoid(z.y));
         }
       }
     __syncthreads();
     if (k + 1 < kl) fetch(k + 1);
-    float sd = 0.f;
+    F2 sd = 0;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
-      float y[kGroup][1];
+      float y[kGroup][2];
 #pragma unroll
       for (int i = 0; i < kGroup; ++i) {
         const int kk = q * kGroup + i;
-        const float2 dx = stage[w.warp][kk][w.c];
-        const F2 dt2 = f2(dx.x, dx.x), x2 = f2(dx.y, dx.y);
-        const ulonglong2 Bv = *reinterpret_cast<const ulonglong2*>(&sB[buf][kk][w.j * NS]);
-        h01 = fma2(exp2_2(mul2(dt2, A01)), h01, mul2(x2, Bv.x));
-        h23 = fma2(exp2_2(mul2(dt2, A23)), h23, mul2(x2, Bv.y));
+        const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(&sm.stage[w.warp][kk][w.c]);
+        F2 Bn[NS];
+        twice4(Bn, &sm.B[buf][kk][w.j * NS]);
+#pragma unroll
+        for (int m = 0; m < NS; ++m) h[m] = fma2(exp2_2(mul2(s.x, A2[m])), h[m], mul2(s.y, Bn[m]));
         if (AGG) {
-          sd += dx.x;
+          sd = add2(sd, s.x);
         } else {
-          const ulonglong2 Cv = *reinterpret_cast<const ulonglong2*>(&sC[AGG ? 0 : buf][AGG ? 0 : kk][w.j * NS]);
-          y[i][0] = hsum(fma2(Cv.y, h23, mul2(Cv.x, h01)));
+          F2 Cn[NS];
+          twice4(Cn, &sm.C[AGG ? 0 : buf][AGG ? 0 : kk][w.j * NS]);
+          const float2 v = un2(fma2(Cn[3], h[3], fma2(Cn[2], h[2], fma2(Cn[1], h[1], mul2(Cn[0], h[0])))));
+          y[i][0] = v.x;
+          y[i][1] = v.y;
         }
       }
       if (!AGG) {
@@ -154,38 +147,40 @@ __global__ void __launch_bounds__(NT, LPC < 4 ? 3 : MOGT_FWD_CTAS) scan_fwd_kern
 #pragma unroll
         for (int i = 0; i < TPL; ++i) {
           const int kk = q * kGroup + tok + i;
-          float o = fmaf(Dd, u[q][i], y[i][0]);
-          if (gate) o *= gz[q][i];
-          if (kk > live) o = 0.f;
-          if (store && kk < rows) out[(int64_t)kk * D] = from_f32<T>(o);
+          float o0 = fmaf(Dd.x, u[q][i].x, y[i][0]), o1 = fmaf(Dd.y, u[q][i].y, y[i][1]);
+          if (gate) {
+            o0 *= gz[q][i].x;
+            o1 *= gz[q][i].y;
+          }
+          if (kk > live) o0 = o1 = 0.f;
+          if (store && kk < rows) store_two<T, VEC>(out + (int64_t)kk * D, o0, o1, w.ok1);
         }
       }
     }
     out += (int64_t)kTile * D;
-    sdt += sd;
+    if (AGG) {
+      const float2 v = un2(sd);
+      sdt = make_float2(sdt.x + v.x, sdt.y + v.y);
+    }
     __syncwarp();  // the stage is rewritten for the next tile
   }
   if constexpr (AGG) {
-    if (w.ok) {
-      const float2 a = un2(h01), b = un2(h23);
-      const int64_t i = blockIdx.y * p.B * p.D + cell;
-      seg.loc[i * LPC + w.j] = make_float4(a.x, a.y, b.x, b.y);
-      if (w.j == 0) seg.sdt[i] = sdt;
+    const int64_t i = blockIdx.y * p.B * p.D + cell;
+    w.put4(seg.loc + w.j, i, h);
+    if (w.j == 0) {
+      if (w.ok) seg.sdt[i] = sdt.x;
+      if (w.ok1) seg.sdt[i + 1] = sdt.y;
     }
   } else {
     // tiles behind the end
     for (int64_t t = max(kl, k0) * kTile + tok; t < min(k1 * kTile, p.L); t += kGroup)
 #pragma unroll
       for (int i = 0; i < TPL; ++i)
-        if (store && t + i < p.L) static_cast<T*>(p.out)[(w.b * p.L + t + i) * p.D + w.d] = from_f32<T>(0.f);
-    if (p.final_state && w.ok && (int)blockIdx.y == geo.nseg - 1) {
-      const float2 a = un2(h01), b = un2(h23);
-      const float h[NS] = {a.x, a.y, b.x, b.y};
+        if (store && t + i < p.L)
+          store_two<T, VEC>(static_cast<T*>(p.out) + (w.b * p.L + t + i) * p.D + w.d, 0.f, 0.f, w.ok1);
+    if (p.final_state && (int)blockIdx.y == geo.nseg - 1) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const int n = w.j * NS + i;
-        if (n < p.N) p.final_state[cell * p.N + n] = h[i];
-      }
+      for (int i = 0; i < NS; ++i) w.put_state(p.final_state, cell, p.N, w.j * NS + i, h[i]);
     }
   }
 }
@@ -266,7 +261,7 @@ extern "C" size_t mogt_selective_saved_bytes(int64_t B, int64_t L, int64_t D, in
 
 extern "C" size_t mogt_selective_fwd_scratch_bytes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
   if (B <= 0 || L < 0 || D <= 0 || N <= 0 || N > kMaxN || G <= 0 || D % G) return 0;
-  return seg_scratch_bytes(B, D, N, num_segments(B, L, D, N, G, NT, kFwdWarps));
+  return seg_scratch_bytes(B, D, N, fwd_segments(B, L, D, N, G));
 }
 
 extern "C" int mogt_selective_scan_fwd(const mogt_selective_args* args, void* stream) {
@@ -275,21 +270,34 @@ extern "C" int mogt_selective_scan_fwd(const mogt_selective_args* args, void* st
   if (int st = check_args(p)) return st;
   if (p.B == 0 || p.D == 0) return MOGT_OK;
   if (!p.A || (p.L > 0 && (!p.u || !p.delta || !p.Bm || !p.Cm || !p.out))) return MOGT_ERR_ARG;
-  const Geo geo = geometry(p, NT, kFwdWarps);
+  const Geo geo = geometry(p, NT, fwd_segments(p.B, p.L, p.D, p.N, p.G));
   const size_t need = seg_scratch_bytes(p.B, p.D, p.N, geo.nseg);
   if (need && (!p.scratch || p.scratch_bytes < need)) return MOGT_ERR_WORKSPACE;
   if ((reinterpret_cast<uintptr_t>(p.saved) | (need ? reinterpret_cast<uintptr_t>(p.scratch) : 0)) & 15u)
     return MOGT_ERR_ALIGN;
   const SegScratch seg = seg_scratch(p.scratch, p.B, p.D, p.N, geo.nseg);
   cudaStream_t s = (cudaStream_t)stream;
+  const bool vec = pairs_aligned(p, false);
   return dispatch(p.dtype, p.N, [&](auto t, auto l) {
     using T = decltype(t);
     constexpr int LPC = decltype(l)::value;
-    const unsigned gx = (unsigned)(geo.nblk * p.G);
-    if (geo.nseg > 1)
-      scan_fwd_kernel<T, LPC, true><<<dim3(gx, geo.nseg - 1, (unsigned)p.B), NT, 0, s>>>(p, geo, seg);
-    scan_fwd_kernel<T, LPC, false><<<dim3(gx, geo.nseg, (unsigned)p.B), NT, 0, s>>>(p, geo, seg);
-    return mogt_host::launch_status();
+    auto go = [&](auto kern, int bytes, int nseg) {
+      if (bytes > 48 * 1024 &&
+          cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        return false;
+      kern<<<dim3((unsigned)(geo.nblk * p.G), nseg, (unsigned)p.B), NT, bytes, s>>>(p, geo, seg);
+      return true;
+    };
+    bool ok = true;
+    if (geo.nseg > 1) {
+      constexpr int bytes = (int)sizeof(FwdSmem<LPC, true>);
+      ok = vec ? go(scan_fwd_kernel<T, LPC, true, true>, bytes, geo.nseg - 1)
+               : go(scan_fwd_kernel<T, LPC, false, true>, bytes, geo.nseg - 1);
+    }
+    constexpr int bytes = (int)sizeof(FwdSmem<LPC, false>);
+    ok = ok && (vec ? go(scan_fwd_kernel<T, LPC, true, false>, bytes, geo.nseg)
+                    : go(scan_fwd_kernel<T, LPC, false, false>, bytes, geo.nseg));
+    return ok ? mogt_host::launch_status() : (int)MOGT_ERR_LAUNCH;
   });
 }
 

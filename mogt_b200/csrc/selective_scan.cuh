@@ -10,11 +10,8 @@ namespace mogt {
 namespace sel {
 
 constexpr int NT = 128;      // threads per CTA of the forward
-#ifndef MOGT_NTB
-#define MOGT_NTB 256
-#endif
-constexpr int NTB = MOGT_NTB;  // and of the backward
-constexpr int NS = 4;        // states per thread
+constexpr int NTB = 128;     // and of the backward
+constexpr int NS = 4;        // states per thread, of each of its two channels
 constexpr int kGroup = 8;    // tokens handled together by the forward
 constexpr int kGroupB = 4;   // and by the backward
 constexpr int kTile = 16;    // tokens per B/C tile and per saved state
@@ -65,6 +62,19 @@ __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Four values, each for both halves of a register pair (both channels).
+__device__ __forceinline__ void twice4(F2 (&r)[4], const float* p) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  r[0] = f2(v.x, v.x);
+  r[1] = f2(v.y, v.y);
+  r[2] = f2(v.z, v.z);
+  r[3] = f2(v.w, v.w);
+}
 __device__ __forceinline__ F2 exp2_2(F2 a) {
   const float2 v = un2(a);
   return f2(fast_exp2(v.x), fast_exp2(v.y));
@@ -74,10 +84,10 @@ __device__ __forceinline__ float hsum(F2 a) {
   return v.x + v.y;
 }
 
-// Lane = c + CPW * j: channel c of the warp's CPW, part j of its LPC.
+// Lane = c + CPW * j: channel pair c of the warp's CPW, part j of its LPC.
 template <int LPC, int GROUP = kGroup>
 struct Lane {
-  static constexpr int CPW = 32 / LPC;                        // channels per warp
+  static constexpr int CPW = 32 / LPC;                        // channel pairs per warp
   static constexpr int NP = LPC * NS;                         // states, padded
   static constexpr int TPL = LPC >= GROUP ? 1 : GROUP / LPC;  // tokens of a group per lane
   static constexpr int DUP = LPC > GROUP ? LPC / GROUP : 1;   // lanes per token beyond that
@@ -89,12 +99,14 @@ struct Geo {
   int nseg;               // segments per sequence (gridDim.y)
 };
 
-// Channel, group and batch row of a thread.  grid = (nblk * G, segments, B).
+inline int channels_per_cta(int threads, int lpc) { return 2 * threads / lpc; }
+
+// Channels (a pair), group and batch row of a thread.  grid = (nblk * G, segments, B).
 template <int LPC, int GROUP = kGroup>
 struct Where {
   int warp, c, j;
-  int64_t b, g, d;
-  bool ok;
+  int64_t b, g, d;  // d: first channel of the pair (a channel of the group for idle lanes)
+  bool ok, ok1;     // the first and the second channel exist
   __device__ __forceinline__ Where(const mogt_selective_args& p, const Geo& geo) {
     const int lane = threadIdx.x & 31;
     warp = threadIdx.x >> 5;
@@ -102,8 +114,9 @@ struct Where {
     j = lane / Lane<LPC>::CPW;
     b = blockIdx.z;
     g = blockIdx.x / geo.nblk;
-    const int64_t i = (blockIdx.x % geo.nblk) * (int)(blockDim.x / LPC) + warp * Lane<LPC>::CPW + c;
+    const int64_t i = (blockIdx.x % geo.nblk) * (int)(2 * blockDim.x / LPC) + 2 * (warp * Lane<LPC>::CPW + c);
     ok = i < geo.Dg;
+    ok1 = i + 1 < geo.Dg;
     d = g * geo.Dg + (ok ? i : 0);
   }
   // first token of the group that this lane loads, and whether it stores it
@@ -111,31 +124,76 @@ struct Where {
     return LPC >= GROUP ? j / Lane<LPC, GROUP>::DUP : j * Lane<LPC, GROUP>::TPL;
   }
   __device__ __forceinline__ bool owner() const { return Lane<LPC, GROUP>::DUP == 1 || j % Lane<LPC, GROUP>::DUP == 0; }
-};
-
-// A lane's elements of one [B, L, D] operand for one tile: TPL tokens of each
-// group of GROUP.  fetch() only issues the loads.  Tokens behind the end are
-// read from the last live one and cleared where they are used: no load needs
-// a predicate, and an address is one multiply-add.
-template <typename T, int TPL, int GROUP>
-struct TileRaw {
-  T v[kTile / GROUP][TPL];
-  // p: the tile's first token; tok: the lane's first; last: index of the last live token in the tile
-  __device__ __forceinline__ void fetch(const T* p, int sl, int tok, int last) {
-#pragma unroll
-    for (int q = 0; q < kTile / GROUP; ++q)
-#pragma unroll
-      for (int i = 0; i < TPL; ++i) v[q][i] = p[(int64_t)min(q * GROUP + tok + i, last) * sl];
+  // a per-channel parameter, 0 where it is not given
+  __device__ __forceinline__ float2 param(const float* v) const {
+    return v ? make_float2(v[d], v[d + ok1]) : make_float2(0.f, 0.f);
+  }
+  // [D, N] values of state n for both channels, 0 for padded states and missing channels
+  __device__ __forceinline__ F2 state(const float* v, int64_t cell, int64_t N, int n) const {
+    return f2(v && ok && n < N ? v[cell * N + n] : 0.f, v && ok1 && n < N ? v[(cell + 1) * N + n] : 0.f);
+  }
+  __device__ __forceinline__ void put_state(float* v, int64_t cell, int64_t N, int n, F2 x) const {
+    if (n < N) {
+      if (ok) v[cell * N + n] = un2(x).x;
+      if (ok1) v[(cell + 1) * N + n] = un2(x).y;
+    }
+  }
+  // The 4 states of a lane for both channels in [.., D, LPC] float4 arrays (i: first channel's index)
+  __device__ __forceinline__ void put4(float4* v, int64_t i, const F2 (&x)[NS]) const {
+    const float2 a = un2(x[0]), b = un2(x[1]), e = un2(x[2]), f = un2(x[3]);
+    if (ok) v[i * LPC] = make_float4(a.x, b.x, e.x, f.x);
+    if (ok1) v[(i + 1) * LPC] = make_float4(a.y, b.y, e.y, f.y);
   }
 };
 
-// The same for one group of a tile (first token kk of the lane).
-template <typename T, int TPL>
-struct GroupRaw {
-  T v[TPL];
-  __device__ __forceinline__ void fetch(const T* p, int sl, int kk, int last) {
+// Two neighbouring channels' elements.  VEC: one access (pairs aligned);
+// otherwise two (one: distance to the second channel, 0 when there is none).
+template <typename T>
+struct Two {
+  using Raw = typename RawVec<2 * (int)sizeof(T)>::type;
+  union {
+    Raw raw;
+    T e[2];
+  };
+  __device__ __forceinline__ Two() {}
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* p, int one) {
+    if (VEC) {
+      raw = *reinterpret_cast<const Raw*>(p);
+    } else {
+      e[0] = p[0];
+      e[1] = p[one];
+    }
+  }
+  __device__ __forceinline__ float2 f() const { return make_float2(to_f32(e[0]), to_f32(e[1])); }
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_two(T* p, float a, float b, bool second) {
+  Two<T> v;
+  v.e[0] = from_f32<T>(a);
+  v.e[1] = from_f32<T>(b);
+  if (VEC) {
+    *reinterpret_cast<typename Two<T>::Raw*>(p) = v.raw;
+  } else {
+    p[0] = v.e[0];
+    if (second) p[1] = v.e[1];
+  }
+}
+
+// A lane's elements of one [B, L, D] operand for COUNT runs of TPL tokens,
+// GROUP apart.  fetch() only issues the loads.  Tokens behind the end are read
+// from the last live one and cleared where they are used: no load needs a
+// predicate, and an address is one multiply-add.
+template <typename T, int TPL, int GROUP, int COUNT, bool VEC>
+struct Raws {
+  Two<T> v[COUNT][TPL];
+  // p: the tile's first token; tok: the lane's first; last: index of the last live token in the tile
+  __device__ __forceinline__ void fetch(const T* p, int sl, int tok, int last, int one) {
 #pragma unroll
-    for (int i = 0; i < TPL; ++i) v[i] = p[(int64_t)min(kk + i, last) * sl];
+    for (int q = 0; q < COUNT; ++q)
+#pragma unroll
+      for (int i = 0; i < TPL; ++i)
+        v[q][i].template load<VEC>(p + (int64_t)min(q * GROUP + tok + i, last) * sl, one);
   }
 };
 
@@ -165,6 +223,32 @@ struct BcRaw {
   }
 };
 
+// dt and x = dt u of a pair from its raw operands, (0, 0) for dead tokens.
+struct DtX {
+  float2 dt, x;
+};
+__device__ __forceinline__ DtX make_dtx(float2 delta, float2 u, float2 bias, bool sp, bool dead) {
+  DtX r;
+  r.dt = make_float2(delta.x + bias.x, delta.y + bias.y);
+  if (sp) r.dt = make_float2(softplus(r.dt.x), softplus(r.dt.y));
+  r.x = make_float2(r.dt.x * u.x, r.dt.y * u.y);
+  if (dead) r.dt = r.x = make_float2(0.f, 0.f);
+  return r;
+}
+
+// States in XORed order (the backward): slot i of a lane of channel pair c
+// holds state i ^ (c & mask).
+template <int LPC>
+struct Perm {
+  static constexpr int COPIES = Lane<LPC>::CPW >= 4 ? 4 : Lane<LPC>::CPW;
+  static constexpr int MASK = COPIES - 1;
+  __device__ static __forceinline__ float4 apply(float4 v, int c) {
+    if (COPIES > 1 && (c & 1)) v = make_float4(v.y, v.x, v.w, v.z);
+    if (COPIES > 2 && (c & 2)) v = make_float4(v.z, v.w, v.x, v.y);
+    return v;
+  }
+};
+
 // Segment carries.  A segment maps the state h entering it to
 // exp(A sum dt) h + loc (loc: its state from zero), a reverse segment the
 // adjoint likewise, so what a segment starts from is a short chain over the
@@ -174,12 +258,24 @@ struct SegScratch {
   float* sdt;   // [nseg - 1][B][D]
 };
 
-template <int LPC, typename W>
-__device__ __forceinline__ void load_A(float (&A2)[NS], const mogt_selective_args& p, const W& w) {
-#pragma unroll
-  for (int i = 0; i < NS; ++i) {
-    const int n = w.j * NS + i;
-    A2[i] = (w.ok && n < p.N) ? p.A[w.d * p.N + n] * kLog2e : 0.f;
+// The state (or adjoint) entering a segment: the chain over segments
+// first, first + step, ..., count of them.  x: what the chain starts from.
+template <int LPC, typename W, bool PERM>
+__device__ __forceinline__ void chain(F2 (&x)[NS], const F2 (&A2)[NS], const SegScratch& s, int first, int step,
+                                      int count, int64_t BD, int64_t cell, const W& w) {
+#pragma unroll 2
+  for (int k = 0; k < count; ++k) {
+    const int64_t i = (first + k * step) * BD + cell;
+    float4 l0 = s.loc[i * LPC + w.j], l1 = s.loc[(i + w.ok1) * LPC + w.j];
+    if (PERM) {
+      l0 = Perm<LPC>::apply(l0, w.c);
+      l1 = Perm<LPC>::apply(l1, w.c);
+    }
+    const F2 sd = f2(s.sdt[i], s.sdt[i + w.ok1]);
+    x[0] = fma2(exp2_2(mul2(sd, A2[0])), x[0], f2(l0.x, l1.x));
+    x[1] = fma2(exp2_2(mul2(sd, A2[1])), x[1], f2(l0.y, l1.y));
+    x[2] = fma2(exp2_2(mul2(sd, A2[2])), x[2], f2(l0.z, l1.z));
+    x[3] = fma2(exp2_2(mul2(sd, A2[3])), x[3], f2(l0.w, l1.w));
   }
 }
 
@@ -191,7 +287,6 @@ __device__ __forceinline__ void sum_parts(float (&v)[GROUP][M], int j) {
 #pragma unroll
   for (int bit = LPC / 2; bit > 0; bit >>= 1) {
     const bool hi = j & bit;
-    const int off = bit * Lane<LPC>::CPW;
     if (n > 1) {
       n >>= 1;
 #pragma unroll
@@ -201,11 +296,11 @@ __device__ __forceinline__ void sum_parts(float (&v)[GROUP][M], int j) {
           for (int m = 0; m < M; ++m) {
             const float send = hi ? v[i][m] : v[i + n][m];
             const float keep = hi ? v[i + n][m] : v[i][m];
-            v[i][m] = keep + __shfl_xor_sync(0xffffffffu, send, off);
+            v[i][m] = keep + __shfl_xor_sync(0xffffffffu, send, bit * Lane<LPC>::CPW);
           }
     } else {
 #pragma unroll
-      for (int m = 0; m < M; ++m) v[0][m] += __shfl_xor_sync(0xffffffffu, v[0][m], off);
+      for (int m = 0; m < M; ++m) v[0][m] += __shfl_xor_sync(0xffffffffu, v[0][m], bit * Lane<LPC>::CPW);
     }
   }
 }
@@ -218,28 +313,62 @@ inline int lpc_of(int64_t N) {
 
 // Segments: the scan over one sequence is serial, so when channels and
 // sequences alone do not fill the GPU the tiles are split into segments, at
-// the price of a first pass over all but one of them (states from zero; about
-// `cost` of the main pass).  Warps wanted: `warps_per_sm` on 148 SMs.
-inline int64_t num_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G, int threads, int warps_per_sm) {
-  const int64_t cpb = threads / lpc_of(N);
-  const int64_t warps = B * G * ((D / G + cpb - 1) / cpb) * (threads / 32);
-  const int64_t nck = (L + kTile - 1) / kTile;
-  int64_t s = (148 * (int64_t)warps_per_sm) / (warps > 0 ? warps : 1);
-  if (s > nck / 4) s = nck / 4;  // a segment shorter than 4 tiles spends its time starting
-  if (s > 64) s = 64;
-  return s < 2 ? 1 : s;
+// the price of a first pass over all but one of them.  Of 1..64 segments (no
+// shorter than 4 tiles) the count with the least estimated time is taken: a
+// pass over a segment costs its length per wave of CTAs (`slots` resident at
+// once), the first pass `agg` of that.
+inline int64_t num_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G, int threads, int slots, float agg) {
+  const int64_t cpb = channels_per_cta(threads, lpc_of(N));
+  const int64_t ctas = B * G * ((D / G + cpb - 1) / cpb), nck = (L + kTile - 1) / kTile;
+  int64_t best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= 64 && s * 4 <= nck; ++s) {
+    // a full wave runs at the full rate; a partly filled one gains little per missing CTA
+    auto waves = [&](int64_t n) {
+      const double full = (double)(n / slots), rest = (double)(n % slots) / slots;
+      return full + (rest > 0 ? 0.5 + 0.5 * rest : 0.0);
+    };
+    const double t = (waves(ctas * s) + agg * waves(ctas * (s - 1))) / (double)s + 0.002 * (double)s;
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
 }
 
-inline Geo geometry(const mogt_selective_args& p, int threads, int warps_per_sm) {
+inline Geo geometry(const mogt_selective_args& p, int threads, int64_t segments) {
   Geo g;
   g.Dg = p.D / p.G;
-  const int64_t cpb = threads / lpc_of(p.N);
+  const int64_t cpb = channels_per_cta(threads, lpc_of(p.N));
   g.nblk = (g.Dg + cpb - 1) / cpb;
   g.nck = (p.L + kTile - 1) / kTile;
-  const int64_t s = num_segments(p.B, p.L, p.D, p.N, p.G, threads, warps_per_sm);
-  g.tps = (g.nck + s - 1) / s;
+  g.tps = (g.nck + segments - 1) / segments;
   g.nseg = g.nck > 0 ? (int)((g.nck + g.tps - 1) / g.tps) : 1;
   return g;
+}
+
+// Pairs of channels can be accessed at once: even group width, row strides
+// and sequence strides, and bases aligned to a pair.
+inline bool pairs_aligned(const mogt_selective_args& p, bool backward) {
+  const uintptr_t a = p.dtype == MOGT_DTYPE_F32 ? 8 : 4;
+  bool ok = (p.D / p.G) % 2 == 0;
+  auto strided = [&](const void* q, int64_t sb, int64_t sl) {
+    if (q) ok = ok && reinterpret_cast<uintptr_t>(q) % a == 0 && sb % 2 == 0 && sl % 2 == 0;
+  };
+  auto dense = [&](const void* q) { ok = ok && reinterpret_cast<uintptr_t>(q) % a == 0; };
+  strided(p.u, p.u_sb, p.u_sl);
+  strided(p.delta, p.delta_sb, p.delta_sl);
+  strided(p.z, p.z_sb, p.z_sl);
+  if (backward) {
+    strided(p.dout, p.dout_sb, p.dout_sl);
+    dense(p.du);
+    dense(p.ddelta);
+    dense(p.dz);
+  } else {
+    dense(p.out);
+  }
+  return ok;
 }
 
 inline size_t seg_scratch_bytes(int64_t B, int64_t D, int64_t N, int64_t nseg) {
