@@ -140,15 +140,20 @@ def launch(name: str, device: torch.device, *args) -> None:
     pointers and no context manager when the device is already current: the
     single-token calls are bound by the host, and this form costs a few
     microseconds less than the ones below."""
-    fn = getattr(lib(), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(lib(), name)
     index = device.index
     if index == torch.cuda.current_device():
         st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
             st = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if st != OK:
+    if st:
         check(st, name)
+
+
+_fns = {}
 
 
 class tag:

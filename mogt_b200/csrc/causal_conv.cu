@@ -2,12 +2,15 @@
 //   pre_t = b + sum_j w_j x_{t-K+1+j},   y_t = silu(pre_t)
 // and its gradients, with g_t = dy_t act'(pre_t):
 //   dx_t = sum_j w_j g_{t+K-1-j},  dw_j = sum_t g_t x_{t-K+1+j},  db = sum_t g_t.
-// About ten operations per 2- or 4-byte element each way, so HBM bounds it:
-// every element of x (and dy) should be read once and of y (dx) written once.
-// A thread keeps VEC neighbouring channels (one access of up to 16 bytes) and
-// walks RUN consecutive tokens with the last K-1 inputs in registers; only
-// the K-1 rows before a run are read twice (K-1 rows after it as well in the
-// backward, which needs g of the following tokens).
+// About ten (forward) and thirty (backward) operations per 2- or 4-byte
+// element, so HBM bounds it: every element of x (and dy) should be read once
+// and of y (dx) written once.  A thread keeps VEC neighbouring channels (one
+// access of up to 16 bytes, 8 in the backward, which holds three times the
+// registers per channel) and walks a run of consecutive tokens with the last
+// K-1 inputs in registers.  The run's tokens are taken UNR at a time, all
+// their loads issued first: a few kilobytes in flight per warp is what keeps
+// HBM busy.  Only the K-1 rows before a run are read twice (in the backward
+// K-1 rows after it as well, for the g of the following tokens).
 #include "selective.cuh"
 
 namespace mogt {
@@ -21,8 +24,8 @@ struct Params {
   void *y, *fin, *dx, *dinit;
   float* part;  // [runs * B][K + 1][D] partial sums of dw, db
   int64_t x_sb, x_sl, dy_sb, dy_sl;
-  int64_t B, L, D;
-  int run;      // tokens per run
+  int64_t B, L, D, runs;  // runs per sequence
+  int run;                // tokens per run
   int silu, pcode;
 };
 
@@ -34,13 +37,27 @@ __device__ __forceinline__ void hist(Pack<T, VEC>& v, const Params& p, int64_t b
   else v.zero();
 }
 
+// Thread -> (sequence, run, channels): channels fastest.
+struct Spot {
+  int64_t b, run, d;
+  bool ok;
+  __device__ __forceinline__ Spot(const Params& p, int vec) {
+    const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x, cols = p.D / vec;
+    ok = i < cols * p.runs * p.B;
+    d = i % cols * vec;
+    run = i / cols % p.runs;
+    b = i / cols / p.runs;
+  }
+};
+
 template <typename T, int VEC, int K>
-__global__ void __launch_bounds__(NT) fwd_kernel(const Params p) {
-  const int64_t d = ((int64_t)blockIdx.x * NT + threadIdx.x) * VEC;
-  const int64_t b = blockIdx.z;
-  if (d >= p.D) return;
+__global__ void __launch_bounds__(NT, 4) fwd_kernel(const Params p) {
+  constexpr int UNR = 8;
+  const Spot at(p, VEC);
+  if (!at.ok) return;
+  const int64_t b = at.b, d = at.d;
   const int64_t len = seq_len(p.lengths, b, p.L);
-  const int64_t t0 = (int64_t)blockIdx.y * p.run, t1 = min(t0 + p.run, p.L);
+  const int64_t t0 = at.run * p.run, t1 = min(t0 + p.run, p.L);
   if (p.fin && t0 == 0) {
 #pragma unroll
     for (int i = 0; i < K - 1; ++i) {
@@ -49,58 +66,60 @@ __global__ void __launch_bounds__(NT) fwd_kernel(const Params p) {
       v.store(static_cast<T*>(p.fin) + (b * (K - 1) + i) * p.D + d);
     }
   }
-  float w[K][VEC], bias[VEC], h[K][VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-    for (int j = 0; j < K; ++j) w[j][i] = ld_param(p.w, p.pcode, (d + i) * K + j);
-    bias[i] = p.bias ? ld_param(p.bias, p.pcode, d + i) : 0.f;
-  }
-  T* y = static_cast<T*>(p.y) + (b * p.L) * p.D + d;
+  T* y = static_cast<T*>(p.y) + (b * p.L + t0) * p.D + d;
   const int64_t te = min(t1, len);
   if (t0 < te) {
+    float w[K][VEC], bias[VEC];
 #pragma unroll
-    for (int j = 1; j < K; ++j) {
-      Pack<T, VEC> v;
-      hist<T, VEC, K>(v, p, b, t0 - K + j, d);
+    for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) h[j][i] = v.f(i);
+      for (int j = 0; j < K; ++j) w[j][i] = ld_param(p.w, p.pcode, (d + i) * K + j);
+      bias[i] = p.bias ? ld_param(p.bias, p.pcode, d + i) : 0.f;
     }
-    const T* x = static_cast<const T*>(p.x) + b * p.x_sb + d;
-    for (int64_t t = t0; t < te; ++t) {
-      Pack<T, VEC> v, o;
-      v.load(x + t * p.x_sl);
+    // h[0..K-2]: the K-1 tokens before the block, then the block's
+    Pack<T, VEC> h[K - 1 + UNR];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        float s = bias[i];
+    for (int j = 0; j < K - 1; ++j) hist<T, VEC, K>(h[j], p, b, t0 - (K - 1) + j, d);
+    const T* x = static_cast<const T*>(p.x) + b * p.x_sb + t0 * p.x_sl + d;
+    for (int64_t t = t0; t < te; t += UNR) {
+      const int n = (int)min(te - t, (int64_t)UNR);
 #pragma unroll
-        for (int j = 0; j + 1 < K; ++j) {
-          h[j][i] = h[j + 1][i];
-          s = fmaf(w[j][i], h[j][i], s);
+      for (int r = 0; r < UNR; ++r) h[K - 1 + r].load(x + min(r, n - 1) * p.x_sl);
+#pragma unroll
+      for (int r = 0; r < UNR; ++r) {
+        Pack<T, VEC> o;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float s = bias[i];
+#pragma unroll
+          for (int j = 0; j < K; ++j) s = fmaf(w[j][i], h[r + j].f(i), s);
+          o.set(i, p.silu ? s * sigmoid(s) : s);
         }
-        h[K - 1][i] = v.f(i);
-        s = fmaf(w[K - 1][i], h[K - 1][i], s);
-        o.set(i, p.silu ? s * sigmoid(s) : s);
+        if (r < n) o.store(y + r * p.D);
       }
-      o.store(y + t * p.D);
+#pragma unroll
+      for (int j = 0; j < K - 1; ++j) h[j] = h[UNR + j];
+      x += UNR * p.x_sl;
+      y += UNR * p.D;
     }
   }
   Pack<T, VEC> zero;
   zero.zero();
-  for (int64_t t = max(te, t0); t < t1; ++t) zero.store(y + t * p.D);
+  for (int64_t t = max(te, t0); t < t1; ++t) zero.store(static_cast<T*>(p.y) + (b * p.L + t) * p.D + d);
 }
 
 // Walks t from t0 to t1 + K - 2: g_t of the run's own tokens and of the K-1
 // after it; dx_{t-K+1} is complete once g_t is known.  The first run also
 // emits the rows -(K-1)..-1, the gradients of the initial state.
 template <typename T, int VEC, int K>
-__global__ void __launch_bounds__(NT) bwd_kernel(const Params p) {
-  const int64_t d = ((int64_t)blockIdx.x * NT + threadIdx.x) * VEC;
-  const int64_t b = blockIdx.z;
-  if (d >= p.D) return;
+__global__ void __launch_bounds__(NT, 4) bwd_kernel(const Params p) {
+  constexpr int UNR = 4;
+  const Spot at(p, VEC);
+  if (!at.ok) return;
+  const int64_t b = at.b, d = at.d;
   const int64_t len = seq_len(p.lengths, b, p.L);
-  const int64_t t0 = (int64_t)blockIdx.y * p.run, t1 = min(t0 + p.run, p.L);
-  float w[K][VEC], bias[VEC], h[K][VEC], g[K][VEC], dw[K][VEC], db[VEC];
+  const int64_t t0 = at.run * p.run, t1 = min(t0 + p.run, p.L);
+  float w[K][VEC], bias[VEC], g[K][VEC], dw[K][VEC], db[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
 #pragma unroll
@@ -114,78 +133,77 @@ __global__ void __launch_bounds__(NT) bwd_kernel(const Params p) {
   const T* x = static_cast<const T*>(p.x) + b * p.x_sb + d;
   const T* dy = static_cast<const T*>(p.dy) + b * p.dy_sb + d;
   T* dx = static_cast<T*>(p.dx) + (b * p.L) * p.D + d;
+  Pack<T, VEC> h[K - 1 + UNR], gy[UNR];
   if (t0 < len) {
 #pragma unroll
-    for (int j = 1; j < K; ++j) {
-      Pack<T, VEC> v;
-      hist<T, VEC, K>(v, p, b, t0 - K + j, d);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) h[j][i] = v.f(i);
-    }
+    for (int j = 0; j < K - 1; ++j) hist<T, VEC, K>(h[j], p, b, t0 - (K - 1) + j, d);
   }
   const int64_t first = t0 == 0 ? -(int64_t)(K - 1) : t0;  // first row emitted
-  for (int64_t t = t0; t < t1 + K - 1; ++t) {
+  for (int64_t t = t0; t < t1 + K - 1; t += UNR) {
     // rows behind the end carry no gradient
-    const bool live = t < len;
-    Pack<T, VEC> v, gy;
-    if (live) {
-      v.load(x + t * p.x_sl);
-      gy.load(dy + t * p.dy_sl);
-    }
-    const bool mine = t < t1;
-    const int64_t tau = t - (K - 1);
-    const bool emit = tau >= first;
-    Pack<T, VEC> o, df;
-    const int64_t fi = tau - (len - (K - 1));
-    const bool has_f = p.dfinal && fi >= 0 && fi < K - 1;
-    if (emit && has_f) df.load(static_cast<const T*>(p.dfinal) + (b * (K - 1) + fi) * p.D + d);
+    const int n = (int)max(min(len - t, (int64_t)UNR), (int64_t)0);
+    if (n > 0) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-      for (int j = 0; j + 1 < K; ++j) {
-        g[j][i] = g[j + 1][i];
-        h[j][i] = h[j + 1][i];
+      for (int r = 0; r < UNR; ++r) {
+        h[K - 1 + r].load(x + (t + min(r, n - 1)) * p.x_sl);
+        gy[r].load(dy + (t + min(r, n - 1)) * p.dy_sl);
       }
-      float gt = 0.f;
-      if (live) {
-        h[K - 1][i] = v.f(i);
-        float s = bias[i];
+    }
 #pragma unroll
-        for (int j = 0; j < K; ++j) s = fmaf(w[j][i], h[j][i], s);
-        gt = gy.f(i);
+    for (int r = 0; r < UNR; ++r) {
+      const bool live = r < n, mine = t + r < t1;
+      const int64_t tau = t + r - (K - 1), fi = tau - (len - (K - 1));
+      const bool emit = tau >= first && tau < t1;
+      Pack<T, VEC> o, df;
+      const bool has_f = p.dfinal && emit && fi >= 0 && fi < K - 1;
+      if (has_f) df.load(static_cast<const T*>(p.dfinal) + (b * (K - 1) + fi) * p.D + d);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+        for (int j = 0; j + 1 < K; ++j) g[j][i] = g[j + 1][i];
+        float hv[K], s = bias[i];
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+          hv[j] = h[r + j].f(i);
+          s = fmaf(w[j][i], hv[j], s);
+        }
+        float gt = gy[r].f(i);
         if (p.silu) {
           const float sg = sigmoid(s);
           gt *= sg * (1.f + s * (1.f - sg));
         }
-        if (mine) {
+        if (!live) gt = 0.f;
+        if (live && mine) {
 #pragma unroll
-          for (int j = 0; j < K; ++j) dw[j][i] = fmaf(gt, h[j][i], dw[j][i]);
+          for (int j = 0; j < K; ++j) dw[j][i] = fmaf(gt, hv[j], dw[j][i]);
           db[i] += gt;
         }
-      }
-      g[K - 1][i] = gt;
-      // g[m] = g_{tau + m}: dx_tau = sum_j w_j g_{tau + K - 1 - j}
-      float s = 0.f;
+        g[K - 1][i] = gt;
+        // g[m] = g_{tau + m}: dx_tau = sum_j w_j g_{tau + K - 1 - j}
+        float v = 0.f;
 #pragma unroll
-      for (int j = 0; j < K; ++j) s = fmaf(w[j][i], g[K - 1 - j][i], s);
-      if (has_f) s += emit ? df.f(i) : 0.f;
-      o.set(i, s);
-    }
-    if (emit) {
-      if (tau >= 0) {
-        if (tau >= len) o.zero();
-        o.store(dx + tau * p.D);
-      } else if (p.dinit) {
-        o.store(static_cast<T*>(p.dinit) + (b * (K - 1) + (K - 1 + tau)) * p.D + d);
+        for (int j = 0; j < K; ++j) v = fmaf(w[j][i], g[K - 1 - j][i], v);
+        if (has_f) v += df.f(i);
+        o.set(i, v);
+      }
+      if (emit) {
+        if (tau >= 0) {
+          if (tau >= len) o.zero();
+          o.store(dx + tau * p.D);
+        } else if (p.dinit) {
+          o.store(static_cast<T*>(p.dinit) + (b * (K - 1) + (K - 1 + tau)) * p.D + d);
+        }
       }
     }
+#pragma unroll
+    for (int j = 0; j < K - 1; ++j) h[j] = h[UNR + j];
   }
-  float* part = p.part + ((int64_t)b * gridDim.y + blockIdx.y) * (K + 1) * p.D;
+  float* part = p.part + (b * p.runs + at.run) * (K + 1) * p.D + d;
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) part[j * p.D + d + i] = dw[j][i];
-    part[K * p.D + d + i] = db[i];
+    for (int j = 0; j < K; ++j) part[j * p.D + i] = dw[j][i];
+    part[K * p.D + i] = db[i];
   }
 }
 
@@ -198,6 +216,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const float* part, int64_t 
   const int64_t cols = (K + 1) * D;
   float s = 0.f;
   if (col < cols)
+#pragma unroll 8
     for (int64_t r = grp; r < rows; r += 8) s += part[r * cols + col];
   sm[grp][threadIdx.x & 31] = s;
   __syncthreads();
@@ -235,24 +254,21 @@ __global__ void __launch_bounds__(NT) step_kernel(const T* x, int64_t x_sb, cons
   for (int j = 0; j < K - 1; ++j) h[j + 1].store(new_state + (b * (K - 1) + j) * D + d);
 }
 
-// Tokens per run: as many as leave about four waves of CTAs (an HBM-bound
-// kernel wants many loads in flight), between 16 and 128.
+// Tokens per run: about 2400 CTAs (four waves, so that the last one costs
+// little), runs between 24 and 128 tokens: the rows read twice stay few.
 inline int run_len(int64_t B, int64_t L, int64_t D, int vec) {
-  const int64_t cols = (D + (int64_t)NT * vec - 1) / ((int64_t)NT * vec);
-  const int64_t want = 148 * 16;
-  int64_t run = B * L * cols / want;
-  run = run < 16 ? 16 : (run > 128 ? 128 : run);
-  const int64_t least = (L + 65534) / 65535;  // gridDim.y
-  return (int)(run < least ? least : run);
+  int64_t run = B * L * (D / vec) / ((int64_t)2400 * NT);
+  run = run < 24 ? 24 : (run > 128 ? 128 : run);
+  return (int)run;
 }
 inline int64_t num_runs(int64_t L, int run) { return L > 0 ? (L + run - 1) / run : 1; }
 
 inline bool al(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// Widest access that every operand allows: at most 16 bytes, D and all row
+// Widest access that every operand allows: at most `most` bytes, D and all row
 // strides multiples of it, all bases aligned to it.
-inline int pick_vec(int es, int64_t D, const int64_t* strides, int ns, const void* const* ptrs, int np) {
-  for (int v = 16 / es; v > 1; v >>= 1) {
+inline int pick_vec(int most, int es, int64_t D, const int64_t* strides, int ns, const void* const* ptrs, int np) {
+  for (int v = most / es; v > 1; v >>= 1) {
     bool ok = D % v == 0;
     for (int i = 0; i < ns; ++i) ok = ok && strides[i] % v == 0;
     for (int i = 0; i < np; ++i) ok = ok && al(ptrs[i], (size_t)v * es);
@@ -289,7 +305,7 @@ int dispatch_tk(int dtype, int vec, int64_t K, F&& f) {
 
 inline int check(int64_t B, int64_t L, int64_t D, int64_t K, int dtype, int pd) {
   if (B < 0 || L < 0 || D < 0) return MOGT_ERR_SHAPE;
-  if (K < 2 || K > 4 || B > 65535) return MOGT_ERR_UNSUPPORTED;
+  if (K < 2 || K > 4) return MOGT_ERR_UNSUPPORTED;
   if (dtype < 0 || dtype > 2 || pd < 0 || pd > 2) return MOGT_ERR_DTYPE;
   return MOGT_OK;
 }
@@ -312,10 +328,12 @@ extern "C" int mogt_causal_conv_fwd(const void* x, int64_t x_sb, int64_t x_sl, c
   p.x_sb = x_sb; p.x_sl = x_sl; p.B = B; p.L = L; p.D = D; p.silu = silu; p.pcode = param_dtype;
   const int64_t st[2] = {x_sb, x_sl};
   const void* ptrs[4] = {x, init, y, final_state};
-  const int vec = pick_vec(dtype == MOGT_DTYPE_F32 ? 4 : 2, D, st, 2, ptrs, 4);
+  const int vec = pick_vec(16, dtype == MOGT_DTYPE_F32 ? 4 : 2, D, st, 2, ptrs, 4);
   p.run = run_len(B, L, D, vec);
-  const int64_t runs = num_runs(L, p.run);
-  const dim3 grid((unsigned)((D + (int64_t)NT * vec - 1) / ((int64_t)NT * vec)), (unsigned)runs, (unsigned)B);
+  p.runs = num_runs(L, p.run);
+  const int64_t ctas = (B * p.runs * (D / vec) + NT - 1) / NT;
+  if (ctas >= ((int64_t)1 << 31)) return MOGT_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)ctas;
   return dispatch_tk(dtype, vec, K, [&](auto t, auto v, auto k) {
     fwd_kernel<decltype(t), decltype(v)::value, decltype(k)::value><<<grid, NT, 0, (cudaStream_t)stream>>>(p);
     return mogt_host::launch_status();
@@ -326,7 +344,7 @@ extern "C" size_t mogt_causal_conv_bwd_scratch_bytes(int64_t B, int64_t L, int64
   if (B <= 0 || L < 0 || D <= 0) return 0;
   // the narrowest access has the shortest runs
   int64_t most = 0;
-  for (int v = 1; v <= 8; v <<= 1) {
+  for (int v = 1; v <= 4; v <<= 1) {
     const int64_t runs = num_runs(L, run_len(B, L, D, v));
     most = runs > most ? runs : most;
   }
@@ -349,17 +367,24 @@ extern "C" int mogt_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_sl, c
   p.silu = silu; p.pcode = param_dtype;
   const int64_t st[4] = {x_sb, x_sl, dy_sb, dy_sl};
   const void* ptrs[6] = {x, init, dy, dfinal, dx, dinit};
-  const int vec = pick_vec(dtype == MOGT_DTYPE_F32 ? 4 : 2, D, st, 4, ptrs, 6);
+  const int vec = pick_vec(8, dtype == MOGT_DTYPE_F32 ? 4 : 2, D, st, 4, ptrs, 6);
   p.run = run_len(B, L, D, vec);
-  const int64_t runs = num_runs(L, p.run);
-  const dim3 grid((unsigned)((D + (int64_t)NT * vec - 1) / ((int64_t)NT * vec)), (unsigned)runs, (unsigned)B);
+  p.runs = num_runs(L, p.run);
+  const int64_t ctas = (B * p.runs * (D / vec) + NT - 1) / NT;
+  if (ctas >= ((int64_t)1 << 31)) return MOGT_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)ctas;
   cudaStream_t s = (cudaStream_t)stream;
   const int r = dispatch_tk(dtype, vec, K, [&](auto t, auto v, auto k) {
-    bwd_kernel<decltype(t), decltype(v)::value, decltype(k)::value><<<grid, NT, 0, s>>>(p);
-    return mogt_host::launch_status();
+    using T = decltype(t);
+    if constexpr (decltype(v)::value * sizeof(T) <= 8) {
+      bwd_kernel<T, decltype(v)::value, decltype(k)::value><<<grid, NT, 0, s>>>(p);
+      return mogt_host::launch_status();
+    } else {
+      return (int)MOGT_ERR_UNSUPPORTED;  // pick_vec stops at 8 bytes
+    }
   });
   if (r != MOGT_OK) return r;
-  reduce_kernel<<<(unsigned)(((K + 1) * D + 31) / 32), 256, 0, s>>>(p.part, B * runs, D, (int)K, dweight, dbias,
+  reduce_kernel<<<(unsigned)(((K + 1) * D + 31) / 32), 256, 0, s>>>(p.part, B * p.runs, D, (int)K, dweight, dbias,
                                                                     param_dtype);
   return mogt_host::launch_status();
 }
@@ -371,7 +396,7 @@ extern "C" int mogt_causal_conv_step(const void* x, int64_t x_sb, const void* st
   if (B == 0 || D == 0) return MOGT_OK;
   if (!x || !state || !weight || !y || !new_state) return MOGT_ERR_ARG;
   const void* ptrs[4] = {x, state, y, new_state};
-  const int vec = pick_vec(dtype == MOGT_DTYPE_F32 ? 4 : 2, D, &x_sb, 1, ptrs, 4);
+  const int vec = pick_vec(16, dtype == MOGT_DTYPE_F32 ? 4 : 2, D, &x_sb, 1, ptrs, 4);
   const int64_t n = B * (D / vec);
   return dispatch_tk(dtype, vec, K, [&](auto t, auto v, auto k) {
     using T = decltype(t);

@@ -2,13 +2,14 @@
 // policy loss with a KL term, the paired preference loss, and their gradients.
 //   lp = x_l - lse,  lse = m + log sum_v exp(x_v - m);
 //   d lp / d x_v = [v = l] - exp(x_v - lse).
-// One multiply-add, one exponential and a compare or two per logit of 2 or 4
-// bytes: HBM bounds all of it.  A CTA takes a row; the maximum and the sum of
-// exponentials are carried together over one pass (rescaled when the maximum
-// grows).  The policy loss knows a token's coefficient as soon as the row's
-// sum is known, so its gradient row is written by the same CTA at once, while
-// the row it has just read is still in L2: one read and one write of the
-// logits in HBM for the loss and its gradient.
+// About eight operations, one exponential among them, per logit of 2 or 4
+// bytes and pass: HBM bounds all of it.  A CTA takes a row at a time; the
+// maximum and the sum of exponentials are carried together over one pass
+// (rescaled when the maximum grows, once per 4 vectors of 16 bytes, whose
+// loads are issued together).  The policy loss knows a token's coefficient as
+// soon as the row's sum is known, so its gradient row is written by the same
+// CTA at once, while the row it has just read is still in L2: one read and one
+// write of the logits in HBM for the loss and its gradient.
 #include <type_traits>
 
 #include "../../include/mogt_lm_loss.h"
@@ -17,8 +18,11 @@
 namespace mogt {
 namespace lml {
 
-constexpr int NT = 512;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSms = 148, kCtas = 5;  // and small CTAs resident on each
+// Rows up to which every CTA counts the tokens itself (from L2) instead of a
+// launch of its own: 9 bytes a token and CTA.
+constexpr int64_t kInlineCount = 16384;
 
 struct Rows {
   const void* logits;
@@ -36,7 +40,8 @@ struct Policy {
   const float *old, *ref, *adv;
   int64_t adv_sb, adv_sl;
   float lo, hi, kl;
-  const float* inv_n;
+  float* inv_n;
+  bool counted;  // *inv_n is there; otherwise the rows kernel counts
   float *tok, *coef;
 };
 
@@ -76,31 +81,53 @@ struct Split {
   }
 };
 
-// Maximum and sum of exponentials of a row, known to every thread.
-template <typename T>
-__device__ MS row_stats(const T* x, int64_t V, MS* red) {
-  constexpr int VEC = Split<T>::VEC;
-  const Split<T> sp(x, V);
-  float m = -INFINITY, s = 0.f;
-  const T* xv = x + sp.head;
-#pragma unroll 4
-  for (int64_t i = threadIdx.x; i < sp.nvec; i += NT) {
-    Pack<T, VEC> v;
-    v.load(xv + i * VEC);
-    float f[VEC], mx = v.f(0);
+constexpr int UNR = 4;  // 16-byte vectors a thread has in flight
+
+// Vectors i, i + NT, ... of a row; those behind the last hold -inf.
+template <typename T, int NT>
+__device__ __forceinline__ void load_vectors(uint4 (&v)[UNR], const T* xv, int64_t i, int64_t nvec) {
+  const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) {
-      f[k] = v.f(k);
-      mx = fmaxf(mx, f[k]);
-    }
-    const float mn = fmaxf(m, mx);
-    const float ref = mn == -INFINITY ? 0.f : mn;
-    s *= exp_diff(m, ref);
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) s += exp_diff(f[k], ref);
-    m = mn;
+  for (int r = 0; r < UNR; ++r) {
+    const int64_t k = i + (int64_t)r * NT;
+    v[r] = k < nvec ? reinterpret_cast<const uint4*>(xv)[k] : make_uint4(none, none, none, none);
   }
-  MS a{m, s};
+}
+
+// Maximum and sum of exponentials of a row, known to every thread.
+template <typename T, int NT>
+__device__ MS row_stats(const T* x, int64_t V, MS* red) {
+  constexpr int VEC = Split<T>::VEC, W = VEC == 8 ? 1 : 2;  // words per pair
+  const Split<T> sp(x, V);
+  const T* xv = x + sp.head;
+  const F2 l2e = f2(kLog2e, kLog2e);
+  float m = -INFINITY;
+  F2 acc = 0;
+  for (int64_t i = threadIdx.x; i < sp.nvec; i += (int64_t)NT * UNR) {
+    uint4 v[UNR];
+    load_vectors<T, NT>(v, xv, i, sp.nvec);
+    float mx = m;
+#pragma unroll
+    for (int r = 0; r < UNR; ++r)
+#pragma unroll
+      for (int k = 0; k < VEC / 2; ++k) {
+        const float2 f = unpack_two<T>(reinterpret_cast<const uint32_t*>(&v[r]) + k * W);
+        mx = fmaxf(mx, fmaxf(f.x, f.y));
+      }
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    const float sc = exp_diff(m, ref);
+    const F2 neg = f2(-ref, -ref);
+    acc = mul2(acc, f2(sc, sc));
+    m = mx;
+#pragma unroll
+    for (int r = 0; r < UNR; ++r)
+#pragma unroll
+      for (int k = 0; k < VEC / 2; ++k) {
+        const float2 f = unpack_two<T>(reinterpret_cast<const uint32_t*>(&v[r]) + k * W);
+        acc = add2(acc, exp2_2(mul2(add2(f2(f.x, f.y), neg), l2e)));
+      }
+  }
+  MS a{m, hsum(acc)};
   const int64_t edge = threadIdx.x;
   if (edge < sp.head) a = merge(a, one(to_f32(x[edge])));
   if (sp.tail0 + edge < V) a = merge(a, one(to_f32(x[sp.tail0 + edge])));
@@ -119,21 +146,30 @@ __device__ MS row_stats(const T* x, int64_t V, MS* red) {
 }
 
 // d[v] = c * ([v = label] - p_v), p_v = exp(x_v - m) / s.
-template <typename T>
+template <typename T, int NT>
 __device__ void write_grad(const T* x, T* d, int64_t V, int64_t label, float c, float m, float inv_s) {
-  constexpr int VEC = Split<T>::VEC;
+  constexpr int VEC = Split<T>::VEC, W = VEC == 8 ? 1 : 2;
   const Split<T> sp(x, V);
   const float f = -c * inv_s;
   const T* xv = x + sp.head;
   T* dv = d + sp.head;
   if (((reinterpret_cast<uintptr_t>(dv)) & 15u) == 0) {
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < sp.nvec; i += NT) {
-      Pack<T, VEC> v, o;
-      v.load(xv + i * VEC);
+    const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-m, -m), ff = f2(f, f);
+    for (int64_t i = threadIdx.x; i < sp.nvec; i += (int64_t)NT * UNR) {
+      uint4 v[UNR];
+      load_vectors<T, NT>(v, xv, i, sp.nvec);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) o.set(k, f * exp_diff(v.f(k), m));
-      o.store(dv + i * VEC);
+      for (int r = 0; r < UNR; ++r) {
+        uint4 o;
+#pragma unroll
+        for (int k = 0; k < VEC / 2; ++k) {
+          const float2 e = unpack_two<T>(reinterpret_cast<const uint32_t*>(&v[r]) + k * W);
+          const float2 q = un2(mul2(ff, exp2_2(mul2(add2(f2(e.x, e.y), neg), l2e))));
+          pack_two<T>(reinterpret_cast<uint32_t*>(&o) + k * W, q.x, q.y);
+        }
+        const int64_t k = i + (int64_t)r * NT;
+        if (k < sp.nvec) reinterpret_cast<uint4*>(dv)[k] = o;
+      }
     }
   } else {
     for (int64_t i = threadIdx.x; i < sp.nvec * VEC; i += NT) dv[i] = from_f32<T>(f * exp_diff(to_f32(xv[i]), m));
@@ -145,7 +181,7 @@ __device__ void write_grad(const T* x, T* d, int64_t V, int64_t label, float c, 
   if (threadIdx.x == 0 && label < V) d[label] = from_f32<T>(fmaf(f, exp_diff(to_f32(x[label]), m), c));
 }
 
-template <typename T>
+template <typename T, int NT>
 __device__ void write_zero(T* d, int64_t V) {
   constexpr int VEC = Split<T>::VEC;
   const Split<T> sp(d, V);
@@ -159,81 +195,95 @@ __device__ void write_zero(T* d, int64_t V) {
 
 __device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fc00000); }
 
-// One CTA per row: log-probability; with POLICY the token's loss and
-// coefficient, and with GRAD the row of the gradient.
-template <typename T, bool POLICY, bool GRAD>
-__global__ void __launch_bounds__(NT) rows_kernel(const Rows r, const Policy q) {
-  __shared__ MS red[NT / 32];
-  const int64_t row = blockIdx.x, b = row / r.L, l = row % r.L;
-  T* d = GRAD ? static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl : nullptr;
-  if (!counts(r, row)) {
-    if (GRAD) write_zero(d, r.V);
-    if (threadIdx.x == 0) {
-      r.lp[row] = 0.f;
-      if (r.stats) r.stats[row] = make_float2(0.f, 1.f);
-      if (POLICY) q.tok[row] = q.coef[row] = 0.f;
-    }
-    return;
-  }
-  const T* x = static_cast<const T*>(r.logits) + b * r.sb + l * r.sl;
-  const int64_t label = r.labels[row];
-  const MS a = row_stats(x, r.V, red);
-  const float lp = label < r.V ? (to_f32(x[label]) - a.m) - logf(a.s) : nan_f32();
-  float tok = 0.f, c = 0.f;
-  if (POLICY) {
-    const float adv = q.adv[b * q.adv_sb + l * q.adv_sl];
-    const float rr = expf(lp - q.old[row]);
-    const float s1 = rr * adv, s2 = fminf(fmaxf(rr, q.lo), q.hi) * adv;
-    tok = -fminf(s1, s2);
-    c = s1 <= s2 ? -s1 : 0.f;
-    if (s1 != s1) tok = c = s1;  // NaN is not dropped by the minimum
-    if (q.ref) {
-      const float dd = q.ref[row] - lp, e = expm1f(dd);
-      tok = fmaf(q.kl, e - dd, tok);
-      c = fmaf(-q.kl, e, c);
-    }
-    c *= *q.inv_n;
-  }
-  if (threadIdx.x == 0) {
-    r.lp[row] = lp;
-    if (r.stats) r.stats[row] = make_float2(a.m, a.s);
-    if (POLICY) {
-      q.tok[row] = tok;
-      q.coef[row] = c;
-    }
-  }
-  if (GRAD) write_grad(x, d, r.V, label, c, a.m, 1.f / a.s);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(NT) rows_bwd_kernel(const Rows r, const float* coef, int64_t coef_div,
-                                                      const float* scale) {
-  const int64_t row = blockIdx.x, b = row / r.L, l = row % r.L;
-  T* d = static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl;
-  if (!counts(r, row)) {
-    write_zero(d, r.V);
-    return;
-  }
-  float c = coef[row / coef_div];
-  if (scale) c *= *scale;
-  const int64_t label = r.labels[row];
-  if (label >= r.V) c = nan_f32();
-  const float2 st = r.stats[row];
-  write_grad(static_cast<const T*>(r.logits) + b * r.sb + l * r.sl, d, r.V, label, c, st.x, 1.f / st.y);
-}
-
-// 1 / max(number of counting tokens, 1).
-__global__ void __launch_bounds__(1024) count_kernel(const Rows r, float* inv_n) {
-  __shared__ int64_t sm[32];
-  int64_t n = 0;
-  for (int64_t i = threadIdx.x; i < r.rows; i += 1024) n += counts(r, i);
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+// 1 / max(number of counting tokens, 1), by a whole CTA.
+template <int NT>
+__device__ float inverse_count(const Rows& r) {
+  __shared__ int sm[NT / 32];
+  int n = 0;
+#pragma unroll 4
+  for (int64_t i = threadIdx.x; i < r.rows; i += NT) n += counts(r, i);
+  n = __reduce_add_sync(0xffffffffu, n);
   if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = n;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    n = 0;
-    for (int i = 0; i < 32; ++i) n += sm[i];
-    *inv_n = 1.f / (float)(n > 0 ? n : 1);
+  n = 0;
+  for (int i = 0; i < NT / 32; ++i) n += sm[i];
+  return 1.f / (float)(n > 0 ? n : 1);
+}
+
+__global__ void __launch_bounds__(1024) count_kernel(const Rows r, float* inv_n) {
+  const float v = inverse_count<1024>(r);
+  if (threadIdx.x == 0) *inv_n = v;
+}
+
+// A CTA per row (and the rows a grid further on): log-probability; with POLICY
+// the token's loss and coefficient, and with GRAD the row of the gradient.
+template <typename T, int NT, bool POLICY, bool GRAD>
+__global__ void __launch_bounds__(NT, NT == 256 ? kCtas : 1) rows_kernel(const Rows r, const Policy q) {
+  __shared__ MS red[NT / 32];
+  float inv_n = 0.f;
+  if (POLICY) {
+    inv_n = q.counted ? *q.inv_n : inverse_count<NT>(r);
+    if (!q.counted && blockIdx.x == 0 && threadIdx.x == 0) *q.inv_n = inv_n;
+  }
+  for (int64_t row = blockIdx.x; row < r.rows; row += gridDim.x) {
+    const int64_t b = row / r.L, l = row % r.L;
+    T* d = GRAD ? static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl : nullptr;
+    if (!counts(r, row)) {
+      if (GRAD) write_zero<T, NT>(d, r.V);
+      if (threadIdx.x == 0) {
+        r.lp[row] = 0.f;
+        if (r.stats) r.stats[row] = make_float2(0.f, 1.f);
+        if (POLICY) q.tok[row] = q.coef[row] = 0.f;
+      }
+      continue;
+    }
+    const T* x = static_cast<const T*>(r.logits) + b * r.sb + l * r.sl;
+    const int64_t label = r.labels[row];
+    const MS a = row_stats<T, NT>(x, r.V, red);
+    const float lp = label < r.V ? (to_f32(x[label]) - a.m) - logf(a.s) : nan_f32();
+    float tok = 0.f, c = 0.f;
+    if (POLICY) {
+      const float adv = q.adv[b * q.adv_sb + l * q.adv_sl];
+      const float rr = expf(lp - q.old[row]);
+      const float s1 = rr * adv, s2 = fminf(fmaxf(rr, q.lo), q.hi) * adv;
+      tok = -fminf(s1, s2);
+      c = s1 <= s2 ? -s1 : 0.f;
+      if (s1 != s1) tok = c = s1;  // NaN is not dropped by the minimum
+      if (q.ref) {
+        const float dd = q.ref[row] - lp, e = expm1f(dd);
+        tok = fmaf(q.kl, e - dd, tok);
+        c = fmaf(-q.kl, e, c);
+      }
+      c *= inv_n;
+    }
+    if (threadIdx.x == 0) {
+      r.lp[row] = lp;
+      if (r.stats) r.stats[row] = make_float2(a.m, a.s);
+      if (POLICY) {
+        q.tok[row] = tok;
+        q.coef[row] = c;
+      }
+    }
+    if (GRAD) write_grad<T, NT>(x, d, r.V, label, c, a.m, 1.f / a.s);
+  }
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, NT == 256 ? kCtas : 1) rows_bwd_kernel(const Rows r, const float* coef, int64_t coef_div,
+                                                      const float* scale) {
+  for (int64_t row = blockIdx.x; row < r.rows; row += gridDim.x) {
+    const int64_t b = row / r.L, l = row % r.L;
+    T* d = static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl;
+    if (!counts(r, row)) {
+      write_zero<T, NT>(d, r.V);
+      continue;
+    }
+    float c = coef[row / coef_div];
+    if (scale) c *= *scale;
+    const int64_t label = r.labels[row];
+    if (label >= r.V) c = nan_f32();
+    const float2 st = r.stats[row];
+    write_grad<T, NT>(static_cast<const T*>(r.logits) + b * r.sb + l * r.sl, d, r.V, label, c, st.x, 1.f / st.y);
   }
 }
 
@@ -300,6 +350,15 @@ int by_type(int dtype, F&& f) {
   }
 }
 
+// Threads per row and CTAs: small CTAs (several on an SM, each at its own point
+// of a row) when there are rows for them, otherwise one large CTA per row.
+template <typename F>
+int by_rows(int64_t rows, F&& f) {
+  if (rows >= kSms * 2)
+    return f(std::integral_constant<int, 256>{}, (unsigned)(rows < kSms * kCtas ? rows : kSms * kCtas));
+  return f(std::integral_constant<int, 1024>{}, (unsigned)rows);
+}
+
 inline int check(int64_t B, int64_t L, int64_t V, int dtype) {
   if (B < 0 || L < 0 || V <= 0) return MOGT_ERR_SHAPE;
   if (dtype < 0 || dtype > 2) return MOGT_ERR_DTYPE;
@@ -321,8 +380,11 @@ extern "C" int mogt_logprob_fwd(const void* logits, int64_t sb, int64_t sl, cons
   if (!logits || !labels || !logprobs) return MOGT_ERR_ARG;
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, nullptr, 0, 0, logprobs, reinterpret_cast<float2*>(stats)};
   return by_type(dtype, [&](auto t) {
-    rows_kernel<decltype(t), false, false><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, Policy{});
-    return mogt_host::launch_status();
+    return by_rows(r.rows, [&](auto n, unsigned grid) {
+      constexpr int NT = decltype(n)::value;
+      rows_kernel<decltype(t), NT, false, false><<<grid, NT, 0, (cudaStream_t)stream>>>(r, Policy{});
+      return mogt_host::launch_status();
+    });
   });
 }
 
@@ -337,8 +399,11 @@ extern "C" int mogt_logprob_bwd(const void* logits, int64_t sb, int64_t sl, cons
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, nullptr,
          const_cast<float2*>(reinterpret_cast<const float2*>(stats))};
   return by_type(dtype, [&](auto t) {
-    rows_bwd_kernel<decltype(t)><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, coef, coef_div, scale);
-    return mogt_host::launch_status();
+    return by_rows(r.rows, [&](auto n, unsigned grid) {
+      constexpr int NT = decltype(n)::value;
+      rows_bwd_kernel<decltype(t), NT><<<grid, NT, 0, (cudaStream_t)stream>>>(r, coef, coef_div, scale);
+      return mogt_host::launch_status();
+    });
   });
 }
 
@@ -359,15 +424,18 @@ extern "C" int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, cons
   float* inv_n = static_cast<float*>(scratch);
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, logprobs, reinterpret_cast<float2*>(stats)};
   Policy q{old_logprobs, ref_logprobs, adv, adv_sb, adv_sl, 1.f - clip_low, 1.f + clip_high, kl_coef, inv_n,
-           inv_n + 1, coef};
+           r.rows > kInlineCount || r.rows == 0, inv_n + 1, coef};
   cudaStream_t s = (cudaStream_t)stream;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);
-    count_kernel<<<1, 1024, 0, s>>>(r, inv_n);
-    if (r.rows > 0) {
-      if (dlogits) rows_kernel<T, true, true><<<(unsigned)r.rows, NT, 0, s>>>(r, q);
-      else rows_kernel<T, true, false><<<(unsigned)r.rows, NT, 0, s>>>(r, q);
-    }
+    if (q.counted) count_kernel<<<1, 1024, 0, s>>>(r, inv_n);
+    if (r.rows > 0)
+      by_rows(r.rows, [&](auto n, unsigned grid) {
+        constexpr int NT = decltype(n)::value;
+        if (dlogits) rows_kernel<T, NT, true, true><<<grid, NT, 0, s>>>(r, q);
+        else rows_kernel<T, NT, true, false><<<grid, NT, 0, s>>>(r, q);
+        return 0;
+      });
     token_mean_kernel<<<1, 1024, 0, s>>>(q.tok, r.rows, inv_n, loss);
     return mogt_host::launch_status();
   });

@@ -40,33 +40,6 @@ __device__ __forceinline__ float softplus_e(float x, float e) {
 }
 __device__ __forceinline__ float softplus(float x) { return softplus_e(x, exp_neg_abs(x)); }
 
-// Two fp32 in one 64-bit register: one instruction for both halves.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 un2(F2 a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
-}
-__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Four values, each for both halves of a register pair (both channels).
 __device__ __forceinline__ void twice4(F2 (&r)[4], const float* p) {
   const float4 v = *reinterpret_cast<const float4*>(p);
@@ -75,15 +48,6 @@ __device__ __forceinline__ void twice4(F2 (&r)[4], const float* p) {
   r[2] = f2(v.z, v.z);
   r[3] = f2(v.w, v.w);
 }
-__device__ __forceinline__ F2 exp2_2(F2 a) {
-  const float2 v = un2(a);
-  return f2(fast_exp2(v.x), fast_exp2(v.y));
-}
-__device__ __forceinline__ float hsum(F2 a) {
-  const float2 v = un2(a);
-  return v.x + v.y;
-}
-
 // Lane = c + CPW * j: channel pair c of the warp's CPW, part j of its LPC.
 template <int LPC, int GROUP = kGroup>
 struct Lane {

@@ -39,13 +39,13 @@ _MAX_STATES = 128
 
 
 def _cuda(what, *ts):
-    dev = ts[0].device
+    index = ts[0].get_device()   # -1 on the CPU
     for t in ts:
-        if t is not None and not t.is_cuda:
-            raise ValueError(f"{what} requires CUDA tensors")
-        if t is not None and t.device != dev:
+        if t is not None and (index < 0 or t.get_device() != index):
+            if not t.is_cuda or index < 0:
+                raise ValueError(f"{what} requires CUDA tensors")
             raise ValueError(f"{what}: all tensors must be on one device")
-    return dev
+    return ts[0].device
 
 
 _MAX_STRIDE = 1 << 27   # the scan's kernels step over a tile's tokens with 32-bit offsets
@@ -211,27 +211,31 @@ def _grouped(t, what, lead):
 
 
 def _check_scan(what, u, delta, A, Bm, Cm, D, z, delta_bias):
-    lead = tuple(u.shape[:-1])
-    ch = u.shape[-1]
-    if u.dtype not in _DTYPES:
+    """B and C as [..., G, N]; every operand's shape and dtype checked."""
+    shape, dtype = u.shape, u.dtype
+    lead, ch = shape[:-1], shape[-1]
+    if dtype not in _DTYPES:
         raise ValueError(f"{what}: u must be bfloat16, float16 or float32")
     if A.ndim != 2 or A.shape[0] != ch:
         raise ValueError(f"{what}: A must be [D, N]")
-    if not 1 <= A.shape[1] <= _MAX_STATES:
+    n = A.shape[1]
+    if not 1 <= n <= _MAX_STATES:
         raise ValueError(f"{what}: N must be in [1, {_MAX_STATES}]")
-    for name, t in (("delta", delta), ("z", z)):
-        if t is not None and (t.shape != u.shape or t.dtype != u.dtype):
-            raise ValueError(f"{what}: {name} must have u's shape and dtype")
+    if delta.shape != shape or delta.dtype != dtype:
+        raise ValueError(f"{what}: delta must have u's shape and dtype")
+    if z is not None and (z.shape != shape or z.dtype != dtype):
+        raise ValueError(f"{what}: z must have u's shape and dtype")
     Bm, Cm = _grouped(Bm, what, lead), _grouped(Cm, what, lead)
-    if Bm.shape != Cm.shape or Bm.shape[-1] != A.shape[1]:
+    if Bm.shape != Cm.shape or Bm.shape[-1] != n:
         raise ValueError(f"{what}: B and C must have one shape, with A's N states")
-    if Bm.dtype != u.dtype or Cm.dtype != u.dtype:
+    if Bm.dtype != dtype or Cm.dtype != dtype:
         raise ValueError(f"{what}: B and C must have u's dtype")
     if Bm.shape[-2] < 1 or ch % Bm.shape[-2]:
         raise ValueError(f"{what}: the number of channels must be a multiple of the number of groups")
-    for name, t in (("D", D), ("delta_bias", delta_bias)):
-        if t is not None and t.shape != (ch,):
-            raise ValueError(f"{what}: {name} must be [D]")
+    if D is not None and D.shape != (ch,):
+        raise ValueError(f"{what}: D must be [D]")
+    if delta_bias is not None and delta_bias.shape != (ch,):
+        raise ValueError(f"{what}: delta_bias must be [D]")
     return Bm, Cm
 
 
