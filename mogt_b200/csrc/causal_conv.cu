@@ -37,6 +37,33 @@ __device__ __forceinline__ void hist(Pack<T, VEC>& v, const Params& p, int64_t b
   else v.zero();
 }
 
+// The taps and bias of VEC channels.  The parameters' type is looked at once,
+// so that all the loads can be in flight together.
+template <typename P, int VEC, int K>
+__device__ __forceinline__ void load_taps(float (&w)[K][VEC], float (&bias)[VEC], const void* wp, const void* bp,
+                                          int64_t d) {
+  const P* pw = static_cast<const P*>(wp) + d * K;
+  const P* pb = static_cast<const P*>(bp) + d;
+  P rw[K * VEC], rb[VEC];
+#pragma unroll
+  for (int i = 0; i < K * VEC; ++i) rw[i] = pw[i];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) rb[i] = bp ? pb[i] : from_f32<P>(0.f);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) w[j][i] = to_f32(rw[i * K + j]);
+    bias[i] = to_f32(rb[i]);
+  }
+}
+template <int VEC, int K>
+__device__ __forceinline__ void taps(float (&w)[K][VEC], float (&bias)[VEC], const void* wp, const void* bp, int code,
+                                     int64_t d) {
+  if (code == MOGT_DTYPE_F32) load_taps<float, VEC, K>(w, bias, wp, bp, d);
+  else if (code == MOGT_DTYPE_BF16) load_taps<__nv_bfloat16, VEC, K>(w, bias, wp, bp, d);
+  else load_taps<__half, VEC, K>(w, bias, wp, bp, d);
+}
+
 // Thread -> (sequence, run, channels): channels fastest.
 struct Spot {
   int64_t b, run, d;
@@ -70,12 +97,7 @@ __global__ void __launch_bounds__(NT, 4) fwd_kernel(const Params p) {
   const int64_t te = min(t1, len);
   if (t0 < te) {
     float w[K][VEC], bias[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-      for (int j = 0; j < K; ++j) w[j][i] = ld_param(p.w, p.pcode, (d + i) * K + j);
-      bias[i] = p.bias ? ld_param(p.bias, p.pcode, d + i) : 0.f;
-    }
+    taps<VEC, K>(w, bias, p.w, p.bias, p.pcode, d);
     // h[0..K-2]: the K-1 tokens before the block, then the block's
     Pack<T, VEC> h[K - 1 + UNR];
 #pragma unroll
@@ -120,14 +142,11 @@ __global__ void __launch_bounds__(NT, 4) bwd_kernel(const Params p) {
   const int64_t len = seq_len(p.lengths, b, p.L);
   const int64_t t0 = at.run * p.run, t1 = min(t0 + p.run, p.L);
   float w[K][VEC], bias[VEC], g[K][VEC], dw[K][VEC], db[VEC];
+  taps<VEC, K>(w, bias, p.w, p.bias, p.pcode, d);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-      w[j][i] = ld_param(p.w, p.pcode, (d + i) * K + j);
-      g[j][i] = dw[j][i] = 0.f;
-    }
-    bias[i] = p.bias ? ld_param(p.bias, p.pcode, d + i) : 0.f;
+    for (int j = 0; j < K; ++j) g[j][i] = dw[j][i] = 0.f;
     db[i] = 0.f;
   }
   const T* x = static_cast<const T*>(p.x) + b * p.x_sb + d;
@@ -242,11 +261,13 @@ __global__ void __launch_bounds__(NT) step_kernel(const T* x, int64_t x_sb, cons
 #pragma unroll
   for (int j = 0; j < K - 1; ++j) h[j].load(state + (b * (K - 1) + j) * D + d);
   h[K - 1].load(x + b * x_sb + d);
+  float wv[K][VEC], bv[VEC];
+  taps<VEC, K>(wv, bv, w, bias, pcode, d);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    float s = bias ? ld_param(bias, pcode, d + i) : 0.f;
+    float s = bv[i];
 #pragma unroll
-    for (int j = 0; j < K; ++j) s = fmaf(ld_param(w, pcode, (d + i) * K + j), h[j].f(i), s);
+    for (int j = 0; j < K; ++j) s = fmaf(wv[j][i], h[j].f(i), s);
     o.set(i, silu ? s * sigmoid(s) : s);
   }
   o.store(y + b * D + d);
@@ -254,12 +275,13 @@ __global__ void __launch_bounds__(NT) step_kernel(const T* x, int64_t x_sb, cons
   for (int j = 0; j < K - 1; ++j) h[j + 1].store(new_state + (b * (K - 1) + j) * D + d);
 }
 
-// Tokens per run: about 2400 CTAs (four waves, so that the last one costs
-// little), runs between 24 and 128 tokens: the rows read twice stay few.
-inline int run_len(int64_t B, int64_t L, int64_t D, int vec) {
-  int64_t run = B * L * (D / vec) / ((int64_t)2400 * NT);
-  run = run < 24 ? 24 : (run > 128 ? 128 : run);
-  return (int)run;
+// Tokens per run for `waves` waves of the CTAs that are resident at once (4 on
+// each SM), between 24 (the rows read twice stay few) and 512.  The backward
+// takes one wave: a partial row of dw and db is written per run.
+inline int run_len(int64_t B, int64_t L, int64_t D, int vec, int waves) {
+  const int64_t per = (int64_t)148 * 4 * NT * waves, all = B * L * (D / vec);
+  const int64_t run = (all + per - 1) / per;
+  return (int)(run < 24 ? 24 : (run > 512 ? 512 : run));
 }
 inline int64_t num_runs(int64_t L, int run) { return L > 0 ? (L + run - 1) / run : 1; }
 
@@ -329,7 +351,7 @@ extern "C" int mogt_causal_conv_fwd(const void* x, int64_t x_sb, int64_t x_sl, c
   const int64_t st[2] = {x_sb, x_sl};
   const void* ptrs[4] = {x, init, y, final_state};
   const int vec = pick_vec(16, dtype == MOGT_DTYPE_F32 ? 4 : 2, D, st, 2, ptrs, 4);
-  p.run = run_len(B, L, D, vec);
+  p.run = run_len(B, L, D, vec, 2);
   p.runs = num_runs(L, p.run);
   const int64_t ctas = (B * p.runs * (D / vec) + NT - 1) / NT;
   if (ctas >= ((int64_t)1 << 31)) return MOGT_ERR_UNSUPPORTED;
@@ -345,7 +367,7 @@ extern "C" size_t mogt_causal_conv_bwd_scratch_bytes(int64_t B, int64_t L, int64
   // the narrowest access has the shortest runs
   int64_t most = 0;
   for (int v = 1; v <= 4; v <<= 1) {
-    const int64_t runs = num_runs(L, run_len(B, L, D, v));
+    const int64_t runs = num_runs(L, run_len(B, L, D, v, 1));
     most = runs > most ? runs : most;
   }
   return (size_t)(B * most * (K + 1) * D) * sizeof(float);
@@ -368,7 +390,7 @@ extern "C" int mogt_causal_conv_bwd(const void* x, int64_t x_sb, int64_t x_sl, c
   const int64_t st[4] = {x_sb, x_sl, dy_sb, dy_sl};
   const void* ptrs[6] = {x, init, dy, dfinal, dx, dinit};
   const int vec = pick_vec(8, dtype == MOGT_DTYPE_F32 ? 4 : 2, D, st, 4, ptrs, 6);
-  p.run = run_len(B, L, D, vec);
+  p.run = run_len(B, L, D, vec, 1);
   p.runs = num_runs(L, p.run);
   const int64_t ctas = (B * p.runs * (D / vec) + NT - 1) / NT;
   if (ctas >= ((int64_t)1 << 31)) return MOGT_ERR_UNSUPPORTED;

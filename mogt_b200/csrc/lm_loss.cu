@@ -19,10 +19,10 @@ namespace mogt {
 namespace lml {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kSms = 148, kCtas = 5;  // and small CTAs resident on each
-// Rows up to which every CTA counts the tokens itself (from L2) instead of a
-// launch of its own: 9 bytes a token and CTA.
-constexpr int64_t kInlineCount = 16384;
+constexpr int kSms = 148;
+// Rows up to which every CTA counts the tokens itself (9 bytes each, from L2)
+// instead of a launch of its own.
+constexpr int64_t kInlineCount = 1024;
 
 struct Rows {
   const void* logits;
@@ -81,10 +81,18 @@ struct Split {
   }
 };
 
-constexpr int UNR = 4;  // 16-byte vectors a thread has in flight
+// Threads, CTAs on an SM and 16-byte vectors a thread has in flight, chosen by
+// measurement at 8192 x 32000 and 4096 x 32001 bf16: a kernel that reads and
+// rereads its row (the policy loss with its gradient) runs best with 512, 4, 2
+// (163 us; 182 with 256, 6, 4), one that goes over it once with 256, 6, 4
+// (50 and 72 us; 55 and 73).  Few rows get one CTA of 1024 threads each.
+template <int NT>
+struct Tune {
+  static constexpr int kUnroll = NT == 512 ? 2 : 4, kCtas = NT == 256 ? 6 : NT == 512 ? 4 : 1;
+};
 
 // Vectors i, i + NT, ... of a row; those behind the last hold -inf.
-template <typename T, int NT>
+template <typename T, int NT, int UNR>
 __device__ __forceinline__ void load_vectors(uint4 (&v)[UNR], const T* xv, int64_t i, int64_t nvec) {
   const uint32_t none = sizeof(T) == 4 ? 0xff800000u : std::is_same_v<T, __half> ? 0xfc00fc00u : 0xff80ff80u;
 #pragma unroll
@@ -98,6 +106,7 @@ __device__ __forceinline__ void load_vectors(uint4 (&v)[UNR], const T* xv, int64
 template <typename T, int NT>
 __device__ MS row_stats(const T* x, int64_t V, MS* red) {
   constexpr int VEC = Split<T>::VEC, W = VEC == 8 ? 1 : 2;  // words per pair
+  constexpr int UNR = Tune<NT>::kUnroll;
   const Split<T> sp(x, V);
   const T* xv = x + sp.head;
   const F2 l2e = f2(kLog2e, kLog2e);
@@ -105,7 +114,7 @@ __device__ MS row_stats(const T* x, int64_t V, MS* red) {
   F2 acc = 0;
   for (int64_t i = threadIdx.x; i < sp.nvec; i += (int64_t)NT * UNR) {
     uint4 v[UNR];
-    load_vectors<T, NT>(v, xv, i, sp.nvec);
+    load_vectors<T, NT, UNR>(v, xv, i, sp.nvec);
     float mx = m;
 #pragma unroll
     for (int r = 0; r < UNR; ++r)
@@ -148,7 +157,7 @@ __device__ MS row_stats(const T* x, int64_t V, MS* red) {
 // d[v] = c * ([v = label] - p_v), p_v = exp(x_v - m) / s.
 template <typename T, int NT>
 __device__ void write_grad(const T* x, T* d, int64_t V, int64_t label, float c, float m, float inv_s) {
-  constexpr int VEC = Split<T>::VEC, W = VEC == 8 ? 1 : 2;
+  constexpr int VEC = Split<T>::VEC, W = VEC == 8 ? 1 : 2, UNR = Tune<NT>::kUnroll;
   const Split<T> sp(x, V);
   const float f = -c * inv_s;
   const T* xv = x + sp.head;
@@ -157,7 +166,7 @@ __device__ void write_grad(const T* x, T* d, int64_t V, int64_t label, float c, 
     const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-m, -m), ff = f2(f, f);
     for (int64_t i = threadIdx.x; i < sp.nvec; i += (int64_t)NT * UNR) {
       uint4 v[UNR];
-      load_vectors<T, NT>(v, xv, i, sp.nvec);
+      load_vectors<T, NT, UNR>(v, xv, i, sp.nvec);
 #pragma unroll
       for (int r = 0; r < UNR; ++r) {
         uint4 o;
@@ -215,76 +224,74 @@ __global__ void __launch_bounds__(1024) count_kernel(const Rows r, float* inv_n)
   if (threadIdx.x == 0) *inv_n = v;
 }
 
-// A CTA per row (and the rows a grid further on): log-probability; with POLICY
-// the token's loss and coefficient, and with GRAD the row of the gradient.
+// A CTA per row: log-probability; with POLICY the token's loss and
+// coefficient, and with GRAD the row of the gradient.
 template <typename T, int NT, bool POLICY, bool GRAD>
-__global__ void __launch_bounds__(NT, NT == 256 ? kCtas : 1) rows_kernel(const Rows r, const Policy q) {
+__global__ void __launch_bounds__(NT, Tune<NT>::kCtas) rows_kernel(const Rows r, const Policy q) {
   __shared__ MS red[NT / 32];
   float inv_n = 0.f;
   if (POLICY) {
     inv_n = q.counted ? *q.inv_n : inverse_count<NT>(r);
     if (!q.counted && blockIdx.x == 0 && threadIdx.x == 0) *q.inv_n = inv_n;
   }
-  for (int64_t row = blockIdx.x; row < r.rows; row += gridDim.x) {
-    const int64_t b = row / r.L, l = row % r.L;
-    T* d = GRAD ? static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl : nullptr;
-    if (!counts(r, row)) {
-      if (GRAD) write_zero<T, NT>(d, r.V);
-      if (threadIdx.x == 0) {
-        r.lp[row] = 0.f;
-        if (r.stats) r.stats[row] = make_float2(0.f, 1.f);
-        if (POLICY) q.tok[row] = q.coef[row] = 0.f;
-      }
-      continue;
-    }
-    const T* x = static_cast<const T*>(r.logits) + b * r.sb + l * r.sl;
-    const int64_t label = r.labels[row];
-    const MS a = row_stats<T, NT>(x, r.V, red);
-    const float lp = label < r.V ? (to_f32(x[label]) - a.m) - logf(a.s) : nan_f32();
-    float tok = 0.f, c = 0.f;
-    if (POLICY) {
-      const float adv = q.adv[b * q.adv_sb + l * q.adv_sl];
-      const float rr = expf(lp - q.old[row]);
-      const float s1 = rr * adv, s2 = fminf(fmaxf(rr, q.lo), q.hi) * adv;
-      tok = -fminf(s1, s2);
-      c = s1 <= s2 ? -s1 : 0.f;
-      if (s1 != s1) tok = c = s1;  // NaN is not dropped by the minimum
-      if (q.ref) {
-        const float dd = q.ref[row] - lp, e = expm1f(dd);
-        tok = fmaf(q.kl, e - dd, tok);
-        c = fmaf(-q.kl, e, c);
-      }
-      c *= inv_n;
-    }
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / r.L, l = row % r.L;
+  T* d = GRAD ? static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl : nullptr;
+  if (!counts(r, row)) {
+    if (GRAD) write_zero<T, NT>(d, r.V);
     if (threadIdx.x == 0) {
-      r.lp[row] = lp;
-      if (r.stats) r.stats[row] = make_float2(a.m, a.s);
-      if (POLICY) {
-        q.tok[row] = tok;
-        q.coef[row] = c;
-      }
+      r.lp[row] = 0.f;
+      if (r.stats) r.stats[row] = make_float2(0.f, 1.f);
+      if (POLICY) q.tok[row] = q.coef[row] = 0.f;
     }
-    if (GRAD) write_grad<T, NT>(x, d, r.V, label, c, a.m, 1.f / a.s);
+    return;
   }
+  const T* x = static_cast<const T*>(r.logits) + b * r.sb + l * r.sl;
+  const int64_t label = r.labels[row];
+  const MS a = row_stats<T, NT>(x, r.V, red);
+  const float lp = label < r.V ? (to_f32(x[label]) - a.m) - logf(a.s) : nan_f32();
+  float tok = 0.f, c = 0.f;
+  if (POLICY) {
+    const float adv = q.adv[b * q.adv_sb + l * q.adv_sl];
+    const float rr = expf(lp - q.old[row]);
+    const float s1 = rr * adv, s2 = fminf(fmaxf(rr, q.lo), q.hi) * adv;
+    tok = -fminf(s1, s2);
+    c = s1 <= s2 ? -s1 : 0.f;
+    if (s1 != s1) tok = c = s1;  // NaN is not dropped by the minimum
+    if (q.ref) {
+      const float dd = q.ref[row] - lp, e = expm1f(dd);
+      tok = fmaf(q.kl, e - dd, tok);
+      c = fmaf(-q.kl, e, c);
+    }
+    c *= inv_n;
+  }
+  if (threadIdx.x == 0) {
+    r.lp[row] = lp;
+    if (r.stats) r.stats[row] = make_float2(a.m, a.s);
+    if (POLICY) {
+      q.tok[row] = tok;
+      q.coef[row] = c;
+    }
+  }
+  if (GRAD) write_grad<T, NT>(x, d, r.V, label, c, a.m, 1.f / a.s);
 }
 
 template <typename T, int NT>
-__global__ void __launch_bounds__(NT, NT == 256 ? kCtas : 1) rows_bwd_kernel(const Rows r, const float* coef, int64_t coef_div,
+__global__ void __launch_bounds__(NT, Tune<NT>::kCtas) rows_bwd_kernel(const Rows r, const float* coef, int64_t coef_div,
                                                       const float* scale) {
-  for (int64_t row = blockIdx.x; row < r.rows; row += gridDim.x) {
-    const int64_t b = row / r.L, l = row % r.L;
-    T* d = static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl;
-    if (!counts(r, row)) {
-      write_zero<T, NT>(d, r.V);
-      continue;
-    }
-    float c = coef[row / coef_div];
-    if (scale) c *= *scale;
-    const int64_t label = r.labels[row];
-    if (label >= r.V) c = nan_f32();
-    const float2 st = r.stats[row];
-    write_grad<T, NT>(static_cast<const T*>(r.logits) + b * r.sb + l * r.sl, d, r.V, label, c, st.x, 1.f / st.y);
+  const int64_t row = blockIdx.x;
+  const int64_t b = row / r.L, l = row % r.L;
+  T* d = static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl;
+  if (!counts(r, row)) {
+    write_zero<T, NT>(d, r.V);
+    return;
   }
+  float c = coef[row / coef_div];
+  if (scale) c *= *scale;
+  const int64_t label = r.labels[row];
+  if (label >= r.V) c = nan_f32();
+  const float2 st = r.stats[row];
+  write_grad<T, NT>(static_cast<const T*>(r.logits) + b * r.sb + l * r.sl, d, r.V, label, c, st.x, 1.f / st.y);
 }
 
 __device__ double block_sum_1024(double v, double* sm) {
@@ -350,13 +357,9 @@ int by_type(int dtype, F&& f) {
   }
 }
 
-// Threads per row and CTAs: small CTAs (several on an SM, each at its own point
-// of a row) when there are rows for them, otherwise one large CTA per row.
-template <typename F>
+template <int NT, typename F>
 int by_rows(int64_t rows, F&& f) {
-  if (rows >= kSms * 2)
-    return f(std::integral_constant<int, 256>{}, (unsigned)(rows < kSms * kCtas ? rows : kSms * kCtas));
-  return f(std::integral_constant<int, 1024>{}, (unsigned)rows);
+  return rows >= kSms * 2 ? f(std::integral_constant<int, NT>{}) : f(std::integral_constant<int, 1024>{});
 }
 
 inline int check(int64_t B, int64_t L, int64_t V, int dtype) {
@@ -380,9 +383,9 @@ extern "C" int mogt_logprob_fwd(const void* logits, int64_t sb, int64_t sl, cons
   if (!logits || !labels || !logprobs) return MOGT_ERR_ARG;
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, nullptr, 0, 0, logprobs, reinterpret_cast<float2*>(stats)};
   return by_type(dtype, [&](auto t) {
-    return by_rows(r.rows, [&](auto n, unsigned grid) {
+    return by_rows<256>(r.rows, [&](auto n) {
       constexpr int NT = decltype(n)::value;
-      rows_kernel<decltype(t), NT, false, false><<<grid, NT, 0, (cudaStream_t)stream>>>(r, Policy{});
+      rows_kernel<decltype(t), NT, false, false><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, Policy{});
       return mogt_host::launch_status();
     });
   });
@@ -399,9 +402,9 @@ extern "C" int mogt_logprob_bwd(const void* logits, int64_t sb, int64_t sl, cons
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, nullptr,
          const_cast<float2*>(reinterpret_cast<const float2*>(stats))};
   return by_type(dtype, [&](auto t) {
-    return by_rows(r.rows, [&](auto n, unsigned grid) {
+    return by_rows<256>(r.rows, [&](auto n) {
       constexpr int NT = decltype(n)::value;
-      rows_bwd_kernel<decltype(t), NT><<<grid, NT, 0, (cudaStream_t)stream>>>(r, coef, coef_div, scale);
+      rows_bwd_kernel<decltype(t), NT><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, coef, coef_div, scale);
       return mogt_host::launch_status();
     });
   });
@@ -430,10 +433,14 @@ extern "C" int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, cons
     using T = decltype(t);
     if (q.counted) count_kernel<<<1, 1024, 0, s>>>(r, inv_n);
     if (r.rows > 0)
-      by_rows(r.rows, [&](auto n, unsigned grid) {
+      dlogits ? by_rows<512>(r.rows, [&](auto n) {
         constexpr int NT = decltype(n)::value;
-        if (dlogits) rows_kernel<T, NT, true, true><<<grid, NT, 0, s>>>(r, q);
-        else rows_kernel<T, NT, true, false><<<grid, NT, 0, s>>>(r, q);
+        rows_kernel<T, NT, true, true><<<(unsigned)r.rows, NT, 0, s>>>(r, q);
+        return 0;
+      })
+              : by_rows<256>(r.rows, [&](auto n) {
+        constexpr int NT = decltype(n)::value;
+        rows_kernel<T, NT, true, false><<<(unsigned)r.rows, NT, 0, s>>>(r, q);
         return 0;
       });
     token_mean_kernel<<<1, 1024, 0, s>>>(q.tok, r.rows, inv_n, loss);

@@ -1,5 +1,5 @@
-// Shared pieces of the selective state space kernels: loads and stores of
-// VEC consecutive elements as fp32, parameters of a run-time type, the
+// Shared pieces of the selective state space and loss kernels: loads and stores
+// of VEC consecutive elements as fp32, parameters of a run-time type, the
 // activations, packed fp32 pairs.
 #pragma once
 
@@ -69,12 +69,7 @@ struct Pack {
   __device__ __forceinline__ void set(int i, float x) { e[i] = from_f32<T>(x); }
 };
 
-// A parameter array whose element type is known at run time.
-__device__ __forceinline__ float ld_param(const void* p, int code, int64_t i) {
-  if (code == MOGT_DTYPE_F32) return static_cast<const float*>(p)[i];
-  if (code == MOGT_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(static_cast<const __half*>(p)[i]);
-}
+// Store to a parameter array whose element type is known at run time.
 __device__ __forceinline__ void st_param(void* p, int code, int64_t i, float x) {
   if (code == MOGT_DTYPE_F32) static_cast<float*>(p)[i] = x;
   else if (code == MOGT_DTYPE_BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
