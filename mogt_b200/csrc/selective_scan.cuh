@@ -243,9 +243,9 @@ __device__ __forceinline__ void chain(F2 (&x)[NS], const F2 (&A2)[NS], const Seg
   }
 }
 
-// Sums v[0..GROUP-1][M] over the LPC parts of a channel.  Afterwards v[i] holds
+// Sums v[0..GROUP-1][M] over the LPC parts of a channel (STEP lanes apart).  Afterwards v[i] holds
 // token part_tok() + i.  Each halving step exchanges half of what is left.
-template <int LPC, int GROUP, int M>
+template <int LPC, int STEP = 32 / LPC, int GROUP, int M>
 __device__ __forceinline__ void sum_parts(float (&v)[GROUP][M], int j) {
   int n = GROUP;
 #pragma unroll
@@ -260,11 +260,11 @@ __device__ __forceinline__ void sum_parts(float (&v)[GROUP][M], int j) {
           for (int m = 0; m < M; ++m) {
             const float send = hi ? v[i][m] : v[i + n][m];
             const float keep = hi ? v[i + n][m] : v[i][m];
-            v[i][m] = keep + __shfl_xor_sync(0xffffffffu, send, bit * Lane<LPC>::CPW);
+            v[i][m] = keep + __shfl_xor_sync(0xffffffffu, send, bit * STEP);
           }
     } else {
 #pragma unroll
-      for (int m = 0; m < M; ++m) v[0][m] += __shfl_xor_sync(0xffffffffu, v[0][m], bit * Lane<LPC>::CPW);
+      for (int m = 0; m < M; ++m) v[0][m] += __shfl_xor_sync(0xffffffffu, v[0][m], bit * STEP);
     }
   }
 }
