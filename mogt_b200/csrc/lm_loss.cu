@@ -315,25 +315,33 @@ __global__ void __launch_bounds__(1024) token_mean_kernel(const float* tok, int6
 
 __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - log1pf(expf(-fabsf(x))); }
 
-// One CTA: a warp sums a sequence's log-probabilities, a thread takes a pair.
+// One CTA, a warp per pair: the sums of its two sequences and their difference
+// stay in f64 up to the logit (two sums of thousands differ by a few units).
 __global__ void __launch_bounds__(1024) pairs_kernel(const float* lp, const float* ref, int64_t P, int64_t L,
                                                      float beta, float eps, float* loss, float* seq, float* coef) {
   __shared__ double sm[32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int64_t i = w; i < 2 * P; i += 32) {
-    double v = 0.0;
-    for (int64_t l = lane; l < L; l += 32) v += lp[i * L + l];
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) seq[i] = (float)v;
-  }
-  __syncthreads();
   double tot = 0.0;
-  for (int64_t i = threadIdx.x; i < P; i += 1024) {
-    const float x = beta * ((seq[i] - ref[i]) - (seq[P + i] - ref[P + i]));
-    tot -= (1.f - eps) * log_sigmoid(x) + eps * log_sigmoid(-x);
-    const float c = beta / (float)P * (eps / (1.f + expf(-x)) - (1.f - eps) / (1.f + expf(x)));
-    coef[i] = c;
-    coef[P + i] = -c;
+  for (int64_t i = w; i < P; i += 32) {
+    double s[2] = {0.0, 0.0};
+#pragma unroll 4
+    for (int64_t l = lane; l < L; l += 32) {
+      s[0] += lp[i * L + l];
+      s[1] += lp[(P + i) * L + l];
+    }
+    for (int o = 16; o > 0; o >>= 1) {
+      s[0] += __shfl_xor_sync(0xffffffffu, s[0], o);
+      s[1] += __shfl_xor_sync(0xffffffffu, s[1], o);
+    }
+    if (lane == 0) {
+      const float x = (float)((double)beta * ((s[0] - (double)ref[i]) - (s[1] - (double)ref[P + i])));
+      tot -= (1.f - eps) * log_sigmoid(x) + eps * log_sigmoid(-x);
+      const float c = beta / (float)P * (eps / (1.f + expf(-x)) - (1.f - eps) / (1.f + expf(x)));
+      seq[i] = (float)s[0];
+      seq[P + i] = (float)s[1];
+      coef[i] = c;
+      coef[P + i] = -c;
+    }
   }
   tot = block_sum_1024(tot, sm);
   if (threadIdx.x == 0) *loss = (float)(tot / (double)(P > 0 ? P : 1));

@@ -105,6 +105,15 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// sum += x, with the rounding error of the addition collected in lost.
+__device__ __forceinline__ void add_kept(F2& sum, F2& lost, F2 x) {
+  const F2 minus = f2(-1.f, -1.f);
+  const F2 s = add2(sum, x), part = fma2(sum, minus, s);     // what of x arrived
+  const F2 e1 = fma2(fma2(part, minus, s), minus, sum);      // sum - (s - part)
+  const F2 e2 = fma2(part, minus, x);                        // x - part
+  lost = add2(lost, add2(e1, e2));
+  sum = s;
+}
 __device__ __forceinline__ F2 exp2_2(F2 a) {
   const float2 v = un2(a);
   return f2(fast_exp2(v.x), fast_exp2(v.y));

@@ -96,7 +96,7 @@ struct BwdSmem {
   float4 s2[NTB / 32][kTile][Lane<LPC>::CPW];   // (dy, dy', u, u')
   float4 s3[NTB / 32][kTile][Lane<LPC>::CPW];   // softplus' and dout silu'(z), both channels
   float4 hs[kTile / kGroupB - 1][2][NTB];       // states entering the tile's groups but the last
-  float4 sumA[2][NTB];                          // a thread's sums for dA
+  float4 sumA[2][2][NTB];                       // a thread's sums for dA, and what their additions lost
   float red[2][NTB / 32][kTile / 2][2][Lane<LPC>::NP];
 };
 
@@ -256,10 +256,11 @@ __global__ void __launch_bounds__(NTB, LPC == 4 ? MOGT_BWD_CTAS : (LPC == 1 ? 1 
     A2[i] = mul2(w.state(p.A, w.d, p.N, n), l2e);
     cy[i] = w.state(p.dfinal, cell, p.N, n);
   }
-  sm.sumA[0][threadIdx.x] = sm.sumA[1][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sm.sumA[i / 2][i % 2][threadIdx.x] = make_float4(0.f, 0.f, 0.f, 0.f);
   chain<LPC, Where<LPC, kGroupB>, true>(cy, A2, sc.seg, geo.nseg - 2, -1, geo.nseg - 1 - (int)blockIdx.y, p.B * p.D,
                                         cell, w);
-  float2 sumD = make_float2(0.f, 0.f), sumb = make_float2(0.f, 0.f);
+  F2 sumD = 0, lostD = 0, sumb = 0, lostb = 0;
   const float2 Dd = w.param(p.Dskip), bias = w.param(p.bias);
   const bool gate = p.z, sp = p.softplus, store = w.ok && w.owner();
   const int N = (int)p.N, D = (int)p.D, one = w.ok1;
@@ -516,39 +517,49 @@ __global__ void __launch_bounds__(NTB, LPC == 4 ? MOGT_BWD_CTAS : (LPC == 1 ? 1 
       put_copies<T, LPC>(sm.C, rC, N, last_of(k - 1));
       __syncthreads();
     }
-    // tiles' sums first, then their sum: keeps the error of a long sequence small
+    // The sums over a sequence cancel heavily (terms of both signs): a tile's
+    // 16 terms are added as they are, the tiles' sums with what each addition
+    // lost kept beside them.
 #pragma unroll
     for (int m = 0; m < NS; m += 2) {
-      ulonglong2* v = reinterpret_cast<ulonglong2*>(&sm.sumA[m / 2][threadIdx.x]);
-      *v = make_ulonglong2(add2(v->x, tA[m]), add2(v->y, tA[m + 1]));
+      ulonglong2* v = reinterpret_cast<ulonglong2*>(&sm.sumA[m / 2][0][threadIdx.x]);
+      ulonglong2* lost = reinterpret_cast<ulonglong2*>(&sm.sumA[m / 2][1][threadIdx.x]);
+      ulonglong2 sum = *v, l = *lost;
+      add_kept(sum.x, l.x, tA[m]);
+      add_kept(sum.y, l.y, tA[m + 1]);
+      *v = sum;
+      *lost = l;
     }
-    sumD = make_float2(sumD.x + tD.x, sumD.y + tD.y);
-    sumb = make_float2(sumb.x + tb.x, sumb.y + tb.y);
+    add_kept(sumD, lostD, f2(tD.x, tD.y));
+    add_kept(sumb, lostb, f2(tb.x, tb.y));
   }
-  if (!w.owner()) sumD = sumb = make_float2(0.f, 0.f);
+  float2 endD = un2(add2(sumD, lostD)), endb = un2(add2(sumb, lostb));
+  if (!w.owner()) endD = endb = make_float2(0.f, 0.f);
   const int64_t row = blockIdx.y * p.B + w.b;
 #pragma unroll
   for (int i = 0; i < NS; ++i) {
     const int n = w.j * NS + (i ^ cq);
-    w.put_state(sc.dA, row * p.D + w.d, NP, n, reinterpret_cast<const F2*>(&sm.sumA[i / 2][threadIdx.x])[i % 2]);
+    const F2* sum = reinterpret_cast<const F2*>(&sm.sumA[i / 2][0][threadIdx.x]);
+    const F2* lost = reinterpret_cast<const F2*>(&sm.sumA[i / 2][1][threadIdx.x]);
+    w.put_state(sc.dA, row * p.D + w.d, NP, n, add2(sum[i % 2], lost[i % 2]));
     if (p.dinit && blockIdx.y == 0) w.put_state(p.dinit, cell, p.N, n, cy[i]);
   }
 #pragma unroll
   for (int o = CPW; o < 32; o <<= 1) {
-    sumD.x += __shfl_xor_sync(0xffffffffu, sumD.x, o);
-    sumD.y += __shfl_xor_sync(0xffffffffu, sumD.y, o);
-    sumb.x += __shfl_xor_sync(0xffffffffu, sumb.x, o);
-    sumb.y += __shfl_xor_sync(0xffffffffu, sumb.y, o);
+    endD.x += __shfl_xor_sync(0xffffffffu, endD.x, o);
+    endD.y += __shfl_xor_sync(0xffffffffu, endD.y, o);
+    endb.x += __shfl_xor_sync(0xffffffffu, endb.x, o);
+    endb.y += __shfl_xor_sync(0xffffffffu, endb.y, o);
   }
   if (w.j == 0) {
     float* v = sc.dv + row * 2 * p.D + w.d;
     if (w.ok) {
-      v[0] = sumD.x;
-      v[p.D] = sumb.x;
+      v[0] = endD.x;
+      v[p.D] = endb.x;
     }
     if (w.ok1) {
-      v[1] = sumD.y;
-      v[p.D + 1] = sumb.y;
+      v[1] = endD.y;
+      v[p.D + 1] = endb.y;
     }
   }
 }
