@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(NT, LPC < 4 ? 2 : 4) scan_bwd_agg_kernel(const
       F2 Cn[NS];
       twice4(Cn, &sm.C[buf][kk][w.j * NS]);
 #pragma unroll
-      for (int m = 0; m < NS; ++m) g[m] = mul2(exp2_2(mul2(s.x, A2[m])), fma2(Cn[m], s.y, g[m]));
+      for (int m = 0; m < NS; ++m) g[m] = mul2(decay(s.x, A2[m]), fma2(Cn[m], s.y, g[m]));
       sd = add2(sd, s.x);
     }
     const float2 v = un2(sd);
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(NTB, LPC == 4 ? MOGT_BWD_CTAS : (LPC == 1 ? 1 
         F2 Bn[NS];
         twice4(Bn, sm.B[kk][w.j][cq]);
 #pragma unroll
-        for (int m = 0; m < NS; ++m) h[m] = fma2(exp2_2(mul2(s.x, A2[m])), h[m], mul2(s.y, Bn[m]));
+        for (int m = 0; m < NS; ++m) h[m] = fma2(decay(s.x, A2[m]), h[m], mul2(s.y, Bn[m]));
       }
     }
     F2 tA[NS] = {0, 0, 0, 0};
@@ -429,7 +429,7 @@ __global__ void __launch_bounds__(NTB, LPC == 4 ? MOGT_BWD_CTAS : (LPC == 1 ? 1 
         twice4(Bn, sm.B[kq + i][w.j][cq]);
 #pragma unroll
         for (int m = 0; m < NS; ++m) {
-          a[i][m] = exp2_2(mul2(s.x, A2[m]));
+          a[i][m] = decay(s.x, A2[m]);
           hh[i + 1][m] = fma2(a[i][m], hh[i][m], mul2(s.y, Bn[m]));
         }
       }

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(NT, LPC < 4 ? 2 : 4) scan_fwd_kernel(const mog
         F2 Bn[NS];
         twice4(Bn, &sm.B[buf][kk][w.j * NS]);
 #pragma unroll
-        for (int m = 0; m < NS; ++m) h[m] = fma2(exp2_2(mul2(s.x, A2[m])), h[m], mul2(s.y, Bn[m]));
+        for (int m = 0; m < NS; ++m) h[m] = fma2(decay(s.x, A2[m]), h[m], mul2(s.y, Bn[m]));
         if (AGG) {
           sd = add2(sd, s.x);
         } else {
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(NT) step_kernel(const StepParams p) {
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        h[r].e[i] = fmaf(fast_exp2(t * (a.e[i] * kLog2e)), h[r].e[i], x * Bn[r].f(i));
+        h[r].e[i] = fmaf(fast_exp2(fmaf(t, a.e[i] * kLog2e, kExp2Shift)), h[r].e[i], x * Bn[r].f(i));
         s = fmaf(Cn[r].f(i), h[r].e[i], s);
       }
       y[r][0] = s;
