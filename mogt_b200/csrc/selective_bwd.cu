@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(256) reduce_bc_kernel(const mogt_selective_arg
   if (t < seq_len(p.lengths, b, p.L)) {
     const float* src = bc + ((b * p.G + g) * p.L + t) * (2 * NP) + which * NP + n;
     const int64_t stride = p.B * p.G * p.L * 2 * NP;
+#pragma unroll 8
     for (int64_t k = 0; k < nblk; ++k) v += src[k * stride];
   }
   T* dst = static_cast<T*>(which ? p.dC : p.dB);
@@ -591,11 +592,13 @@ __global__ void __launch_bounds__(256) reduce_param_kernel(const mogt_selective_
   if (i < na) {
     const int64_t d = i / p.N, n = i % p.N;
     double v = 0.0;
+#pragma unroll 8
     for (int64_t r = 0; r < rows; ++r) v += sc.dA[(r * p.D + d) * NP + n];
     p.dA[i] = (float)v;
   } else if (i < na + 2 * p.D) {
     const int64_t k = i - na;
     double v = 0.0;
+#pragma unroll 8
     for (int64_t r = 0; r < rows; ++r) v += sc.dv[r * 2 * p.D + k];
     float* dst = k < p.D ? p.dD : p.dbias;
     if (dst) dst[k % p.D] = (float)v;

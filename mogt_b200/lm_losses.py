@@ -135,11 +135,14 @@ class _PolicyLossFn(torch.autograd.Function):
         ctx.save_for_backward(logits, labels, mask, work)
         ctx.grad = d
         ctx.mark_non_differentiable(lp)
+        ctx.set_materialize_grads(False)
         return loss, lp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _glp):
+        if g is None:
+            return (None,) * 9
         d, ctx.grad = ctx.grad, None
         with N.tag("mogt.policy_loss.backward"):
             if d is None:
@@ -157,7 +160,7 @@ class _PolicyLossFn(torch.autograd.Function):
 def _token_f32(what, name, t, shape):
     if t.shape != shape:
         raise ValueError(f"{what}: {name} must be {list(shape)}")
-    return _f32(t.detach())
+    return _f32(t.detach() if t.requires_grad else t)
 
 
 def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, mask=None, clip_low=0.2, clip_high=0.2,
@@ -180,7 +183,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
     ref = None if ref_logprobs is None else _token_f32(what, "ref_logprobs", ref_logprobs, shape)
     if advantages.shape not in (shape, shape[:1]):
         raise ValueError(f"{what}: advantages must be [B] or [B, L]")
-    adv = advantages.detach().to(torch.float32)
+    adv = advantages.detach() if advantages.requires_grad else advantages
+    adv = adv if adv.dtype == torch.float32 else adv.to(torch.float32)
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"{what}: clip_low and clip_high must not be negative")
     if torch.is_grad_enabled() and logits.requires_grad:
@@ -213,11 +217,14 @@ class _PreferenceLossFn(torch.autograd.Function):
             loss, seq, coef, stats = _preference(logits, labels, mask, ref, beta, eps, True)
         ctx.save_for_backward(logits, labels, mask, stats, coef)
         ctx.mark_non_differentiable(seq)
+        ctx.set_materialize_grads(False)
         return loss, seq
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, _gseq):
+        if g is None:
+            return (None,) * 6
         logits, labels, mask, stats, coef = ctx.saved_tensors
         with N.tag("mogt.preference_loss.backward"):
             d = _logprob_bwd(logits, labels, mask, stats.data_ptr(), coef.data_ptr(), max(logits.shape[1], 1), g)

@@ -300,14 +300,17 @@ class _SelectiveScanFn(torch.autograd.Function):
                     None if z is None else torch.zeros_like(u), None if bias is None else torch.zeros_like(bias),
                     None if ctx.init_dtype is None else torch.zeros(B, ch, n, dtype=ctx.init_dtype, device=dev),
                     None, None, None)
-        dout = torch.zeros(B, L, ch, dtype=dt, device=dev) if dout is None else _dense_last(dout.to(dt))
+        if dout is None:
+            dout = torch.zeros(B, L, ch, dtype=dt, device=dev)
+        else:
+            dout = _dense_last(dout if dout.dtype == dt else dout.to(dt))
         dfinal = _f32(dfinal)
         Af, Df, bf = _f32(A), _f32(D), _f32(bias)
         a = _scan_args(u, delta, Af, Bm, Cm, Df, z, bf, None, lengths, ctx.softplus)
-        new = lambda: torch.empty(B, L, ch, dtype=dt, device=dev)
         vec = lambda t: None if t is None else torch.empty(ch, dtype=torch.float32, device=dev)
-        du, ddelta, dz = new(), new(), None if z is None else new()
-        dB, dC = (torch.empty(B, L, G, n, dtype=dt, device=dev) for _ in range(2))
+        du, ddelta = u.new_empty((B, L, ch)), u.new_empty((B, L, ch))
+        dz = None if z is None else u.new_empty((B, L, ch))
+        dB, dC = u.new_empty((B, L, G, n)), u.new_empty((B, L, G, n))
         dA = torch.empty(ch, n, dtype=torch.float32, device=dev)
         dD, dbias = vec(D), vec(bias)
         dinit = None
@@ -322,9 +325,10 @@ class _SelectiveScanFn(torch.autograd.Function):
         a.scratch, a.scratch_bytes = scratch.data_ptr(), nbytes
         with N.tag("mogt.selective_scan.backward"):
             N.launch("mogt_selective_scan_bwd", dev, ctypes.byref(a))
-        cast = lambda g, t: None if g is None else g.to(t.dtype)
+        cast = lambda g, t: g if g is None or t.dtype == torch.float32 else g.to(t.dtype)
         return (du, ddelta, cast(dA, A), dB, dC, cast(dD, D), dz, cast(dbias, bias),
-                None if dinit is None else dinit.to(ctx.init_dtype), None, None, None)
+                dinit if dinit is None or ctx.init_dtype == torch.float32 else dinit.to(ctx.init_dtype),
+                None, None, None)
 
 
 def selective_scan(u, delta, A, B, C, *, D=None, z=None, delta_bias=None, delta_softplus=False, initial_state=None,
