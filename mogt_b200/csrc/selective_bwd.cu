@@ -31,13 +31,13 @@ namespace sel {
 #ifndef MOGT_BWD_WARPS
 #define MOGT_BWD_WARPS 16
 #endif
-#ifndef MOGT_BWD_CTAS
-#define MOGT_BWD_CTAS 3
-#endif
-// Segments of a backward: 3 CTAs fit on an SM; the first pass costs about a
-// quarter of the main one.
+// CTAs on an SM by registers and shared memory.  For 4 lanes per pair (N = 16)
+// three of 168 registers: 355 us at 8192 x 1536, against 427 us for two of 255
+// and 439 us for four of 128, which spill.
+constexpr int bwd_ctas(int lpc) { return lpc == 4 ? 3 : lpc == 1 ? 1 : 2; }
+// The first pass over a split sequence costs about a quarter of the main one.
 inline int64_t bwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
-  return num_segments(B, L, D, N, G, NTB, 148 * MOGT_BWD_CTAS, 0.25f);
+  return num_segments(B, L, D, N, G, NTB, 148 * bwd_ctas(lpc_of(N)), 0.25f);
 }
 
 struct BwdScratch {
@@ -109,7 +109,7 @@ struct AggSmem {
 };
 
 template <typename T, int LPC, bool VEC>
-__global__ void __launch_bounds__(NT, LPC < 4 ? 2 : 4) scan_bwd_agg_kernel(const mogt_selective_args p,
+__global__ void __launch_bounds__(NT, fwd_ctas(LPC)) scan_bwd_agg_kernel(const mogt_selective_args p,
                                                                          const Geo geo, const SegScratch seg) {
   using Q = Lane<LPC>;
   constexpr int TPL = Q::TPL, NP = Q::NP;
@@ -235,7 +235,7 @@ __device__ __forceinline__ void channel_sums(const F2 (&b)[NS], const F2 (&d)[NS
 }
 
 template <typename T, int LPC, bool VEC>
-__global__ void __launch_bounds__(NTB, LPC == 4 ? MOGT_BWD_CTAS : (LPC == 1 ? 1 : 2))
+__global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
     scan_bwd_kernel(const mogt_selective_args p, const Geo geo, const BwdScratch sc) {
   using Q = Lane<LPC, kGroupB>;
   constexpr int CPW = Q::CPW, TPL = Q::TPL, NP = Q::NP, NG = kTile / kGroupB;

@@ -23,10 +23,10 @@
 namespace mogt {
 namespace sel {
 
-// Segments of a forward: 4 CTAs fit on an SM; the first pass costs about 0.7
-// of the main one (310 against 430 us at 32768 x 1536, N = 16).
+// The first pass costs about 0.7 of the main one (320 against 410 us at 32768 x
+// 1536, N = 16).
 inline int64_t fwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
-  return num_segments(B, L, D, N, G, NT, 148 * 4, 0.7f);
+  return num_segments(B, L, D, N, G, NT, 148 * fwd_ctas(lpc_of(N)), 0.7f);
 }
 
 template <int LPC, bool AGG>
@@ -39,7 +39,7 @@ struct FwdSmem {
 // grid = (channel blocks, segments, B).  AGG: the first pass over a split
 // sequence, which leaves each segment's state from zero and its sum of dt.
 template <typename T, int LPC, bool VEC, bool AGG>
-__global__ void __launch_bounds__(NT, LPC < 4 ? 2 : 4) scan_fwd_kernel(const mogt_selective_args p, const Geo geo,
+__global__ void __launch_bounds__(NT, fwd_ctas(LPC)) scan_fwd_kernel(const mogt_selective_args p, const Geo geo,
                                                                        const SegScratch seg) {
   using Q = Lane<LPC>;
   constexpr int TPL = Q::TPL, NP = Q::NP;

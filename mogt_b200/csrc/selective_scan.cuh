@@ -74,6 +74,9 @@ struct Geo {
   int nseg;               // segments per sequence (gridDim.y)
 };
 
+// CTAs of a forward (or first) pass on an SM: fewer lanes per pair hold more
+// tokens each and need more registers.
+constexpr int fwd_ctas(int lpc) { return lpc < 4 ? 2 : 4; }
 inline int channels_per_cta(int threads, int lpc) { return 2 * threads / lpc; }
 
 // Channels (a pair), group and batch row of a thread.  grid = (nblk * G, segments, B).
