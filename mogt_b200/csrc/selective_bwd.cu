@@ -32,7 +32,8 @@ namespace sel {
 #define MOGT_BWD_WARPS 16
 #endif
 // CTAs on an SM by registers and shared memory.  For 4 lanes per pair (N = 16)
-// three of 168 registers: 355 us at 8192 x 1536, against 427 us for two of 255
+// three of 168 registers: 355 us at 8192 x 1536 (before operands were copied
+// asynchronously, 320 us since), against 427 us for two of 255
 // and 439 us for four of 128, which spill.
 constexpr int bwd_ctas(int lpc) { return lpc == 4 ? 3 : lpc == 1 ? 1 : 2; }
 // The first pass over a split sequence costs about a quarter of the main one.
@@ -98,7 +99,18 @@ struct BwdSmem {
   float4 hs[kTile / kGroupB - 1][2][NTB];       // states entering the tile's groups but the last
   float4 sumA[2][2][NTB];                       // a thread's sums for dA, and what their additions lost
   float red[2][NTB / 32][kTile / 2][2][Lane<LPC>::NP];
+  // raw operands of the group and the states of the tile that are on their way, a thread's own
+  uint2 raw[4][Lane<LPC, kGroupB>::TPL][NTB];
+  float4 next[2][NTB];
 };
+
+// Asynchronous copy of BYTES (4, 8 or 16) to this thread's shared memory.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
 // First pass over a split sequence: per segment (all but the first) the
 // adjoint handed to the state before it, from nothing behind it, and sum dt.
@@ -292,8 +304,9 @@ __global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
     }
 
   // Fetching is spread over the groups of the tile before: a group's raw
-  // values are loaded when a group begins and staged when it ends, so few
-  // registers wait on memory.
+  // values are fetched when a group begins and staged when it ends, so little
+  // waits on memory: pairs as asynchronous copies into the thread's own slots
+  // of shared memory, unaligned channels in registers.
   Two<T> ru[TPL], rd[TPL], rz[TPL], ro[TPL];
   BcRaw<T, NP, NTB> rB, rC;
   float4 rs0, rs1;
@@ -303,8 +316,14 @@ __global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
     rC.fetch(Cp + k * kTile * C_sl, C_sl, N, last_of(k));
   };
   auto fetch_saved = [&](int64_t k) {
-    rs0 = saved[k * p.D * LPC];
-    rs1 = saved[(k * p.D + one) * LPC];
+    const float4* v = saved + k * p.D * LPC;
+    if constexpr (VEC) {
+      copy_async<16>(&sm.next[0][threadIdx.x], v);
+      copy_async<16>(&sm.next[1][threadIdx.x], v + one * LPC);
+    } else {
+      rs0 = v[0];
+      rs1 = v[one * LPC];
+    }
   };
   auto fetch = [&](int64_t k, int q) {
     const int64_t t0 = k * kTile;
@@ -312,16 +331,33 @@ __global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
 #pragma unroll
     for (int i = 0; i < TPL; ++i) {
       const int64_t t = t0 + min(q * kGroupB + group_token<LPC>(w.j, i), last);
-      rd[i].template load<VEC>(dp + t * d_sl, one);
-      ru[i].template load<VEC>(up + t * u_sl, one);
-      ro[i].template load<VEC>(op + t * o_sl, one);
-      if (gate) rz[i].template load<VEC>(zp + t * z_sl, one);
+      if constexpr (VEC) {
+        constexpr int PAIR = 2 * (int)sizeof(T);
+        copy_async<PAIR>(&sm.raw[0][i][threadIdx.x], dp + t * d_sl);
+        copy_async<PAIR>(&sm.raw[1][i][threadIdx.x], up + t * u_sl);
+        copy_async<PAIR>(&sm.raw[2][i][threadIdx.x], op + t * o_sl);
+        if (gate) copy_async<PAIR>(&sm.raw[3][i][threadIdx.x], zp + t * z_sl);
+      } else {
+        rd[i].template load<false>(dp + t * d_sl, one);
+        ru[i].template load<false>(up + t * u_sl, one);
+        ro[i].template load<false>(op + t * o_sl, one);
+        if (gate) rz[i].template load<false>(zp + t * z_sl, one);
+      }
     }
+    if constexpr (VEC) copies_issued();
   };
   auto stage = [&](int64_t k, int q) {
     const int live = last_of(k);
+    if constexpr (VEC) copies_landed();
 #pragma unroll
     for (int i = 0; i < TPL; ++i) {
+      if constexpr (VEC) {
+        using R = typename Two<T>::Raw;
+        rd[i].raw = *reinterpret_cast<const R*>(&sm.raw[0][i][threadIdx.x]);
+        ru[i].raw = *reinterpret_cast<const R*>(&sm.raw[1][i][threadIdx.x]);
+        ro[i].raw = *reinterpret_cast<const R*>(&sm.raw[2][i][threadIdx.x]);
+        if (gate) rz[i].raw = *reinterpret_cast<const R*>(&sm.raw[3][i][threadIdx.x]);
+      }
       const int kk = q * kGroupB + group_token<LPC>(w.j, i);
       const float2 uu = ru[i].f(), dd = rd[i].f(), oo = ro[i].f();
       const float2 zz = gate ? rz[i].f() : make_float2(0.f, 0.f);
@@ -377,6 +413,10 @@ __global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
     // states entering the tile's groups wait in shared memory
     F2 h[NS];
     {
+      if constexpr (VEC) {
+        rs0 = sm.next[0][threadIdx.x];
+        rs1 = sm.next[1][threadIdx.x];
+      }
       const float4 a = Perm<LPC>::apply(rs0, w.c), b = Perm<LPC>::apply(rs1, w.c);
       h[0] = f2(w.ok ? a.x : 0.f, w.ok1 ? b.x : 0.f);
       h[1] = f2(w.ok ? a.y : 0.f, w.ok1 ? b.y : 0.f);
@@ -403,11 +443,11 @@ __global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
 #pragma unroll 1
     for (int q = NG - 1; q >= 0; --q) {
       if (k > k0) {
-        fetch(k - 1, q);
         if (q == 0) {
           fetch_bc(k - 1);
-          fetch_saved(k - 1);
+          fetch_saved(k - 1);  // goes with the group's copies
         }
+        fetch(k - 1, q);
       }
       const int kq = q * kGroupB;
       if (q < NG - 1) {
