@@ -39,6 +39,30 @@ def test_prompts_and_tokens_match_the_training_form():
                 assert max_err(logits[b], full[b, n[b] + t]) <= 1e-4, (t, b)
 
 
+def test_a_token_step_in_a_cuda_graph():
+    """A captured step replays on the same buffers like the calls themselves."""
+    m = _model(2)
+    ids = torch.randint(0, 97, (2, 12), device="cuda")
+    _, caches = m.prefill(ids[:, :4])
+    _, want = m.prefill(ids[:, :4])
+    tok = ids[:, 4].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):   # warm-up on copies: a step changes the caches
+        m.step(tok, [tuple(t.clone() for t in c) for c in caches])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        logits = m.step(tok, caches)
+    for t in range(4, 12):
+        tok.copy_(ids[:, t])
+        graph.replay()
+        direct = m.step(ids[:, t], want)
+        assert max_err(logits, direct) <= 1e-6
+        for a, b in zip(caches, want):
+            assert max_err(a[0], b[0]) <= 1e-6 and max_err(a[1], b[1]) <= 1e-6
+
+
 def test_training_gradients_against_float64():
     """Every parameter's gradient of a policy step against the same network in
     float64 (token by token); fp32 projections dominate: 1e-4 relative."""
