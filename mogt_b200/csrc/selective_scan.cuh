@@ -306,7 +306,9 @@ inline int64_t num_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t 
       const double full = (double)(n / slots), rest = (double)(n % slots) / slots;
       return full + (rest > 0 ? 0.5 + 0.5 * rest : 0.0);
     };
-    const double t = (waves(ctas * s) + agg * waves(ctas * (s - 1))) / (double)s + 0.002 * (double)s;
+    // in tiles: starting a segment costs about one, each link of its chain a tenth
+    const double len = (double)((nck + s - 1) / s) + 1.0;
+    const double t = waves(ctas * s) * (len + 0.1 * (double)s) + agg * waves(ctas * (s - 1)) * len;
     if (t < least) {
       least = t;
       best = s;
