@@ -604,30 +604,30 @@ __global__ void __launch_bounds__(NTB, bwd_ctas(LPC))
   }
 }
 
-// dB, dC [B, L, G, N] from the CTAs' partial rows.
+// The partial rows added up, in one launch: CTAs below bc_ctas take dB and dC
+// [B, L, G, N] (over channel blocks), the others dA, dD and dbias (over
+// sequences and segments).
 template <typename T>
-__global__ void __launch_bounds__(256) reduce_bc_kernel(const mogt_selective_args p, int64_t nblk, int NP,
-                                                        const float* bc) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t total = p.B * p.L * p.G * 2 * p.N;
-  if (i >= total) return;
-  const int64_t n = i % p.N, which = (i / p.N) % 2, g = (i / (2 * p.N)) % p.G, bt = i / (2 * p.N * p.G);
-  const int64_t t = bt % p.L, b = bt / p.L;
-  float v = 0.f;
-  if (t < seq_len(p.lengths, b, p.L)) {
-    const float* src = bc + ((b * p.G + g) * p.L + t) * (2 * NP) + which * NP + n;
-    const int64_t stride = p.B * p.G * p.L * 2 * NP;
+__global__ void __launch_bounds__(256) reduce_kernel(const mogt_selective_args p, int64_t nblk, int NP, int64_t rows,
+                                                     int64_t bc_ctas, const BwdScratch sc) {
+  if ((int64_t)blockIdx.x < bc_ctas) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t total = p.B * p.L * p.G * 2 * p.N;
+    if (i >= total) return;
+    const int64_t n = i % p.N, which = (i / p.N) % 2, g = (i / (2 * p.N)) % p.G, bt = i / (2 * p.N * p.G);
+    const int64_t t = bt % p.L, b = bt / p.L;
+    float v = 0.f;
+    if (t < seq_len(p.lengths, b, p.L)) {
+      const float* src = sc.bc + ((b * p.G + g) * p.L + t) * (2 * NP) + which * NP + n;
+      const int64_t stride = p.B * p.G * p.L * 2 * NP;
 #pragma unroll 8
-    for (int64_t k = 0; k < nblk; ++k) v += src[k * stride];
+      for (int64_t k = 0; k < nblk; ++k) v += src[k * stride];
+    }
+    T* dst = static_cast<T*>(which ? p.dC : p.dB);
+    dst[(bt * p.G + g) * p.N + n] = from_f32<T>(v);
+    return;
   }
-  T* dst = static_cast<T*>(which ? p.dC : p.dB);
-  dst[(bt * p.G + g) * p.N + n] = from_f32<T>(v);
-}
-
-// dA, dD, dbias from the partial sums of sequences and segments.
-__global__ void __launch_bounds__(256) reduce_param_kernel(const mogt_selective_args p, int NP, int64_t rows,
-                                                           const BwdScratch sc) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = ((int64_t)blockIdx.x - bc_ctas) * 256 + threadIdx.x;
   const int64_t na = p.D * p.N;
   if (i < na) {
     const int64_t d = i / p.N, n = i % p.N;
@@ -702,10 +702,9 @@ extern "C" int mogt_selective_scan_bwd(const mogt_selective_args* args, void* st
     ok = ok && (vec ? go(scan_bwd_kernel<T, LPC, true>, bytes, geo.nseg, sc)
                     : go(scan_bwd_kernel<T, LPC, false>, bytes, geo.nseg, sc));
     if (!ok) return (int)MOGT_ERR_LAUNCH;
-    const int64_t nbc = p.B * p.L * p.G * 2 * p.N;
-    if (nbc > 0) reduce_bc_kernel<T><<<(unsigned)((nbc + 255) / 256), 256, 0, s>>>(p, geo.nblk, NP, sc.bc);
-    const int64_t np = p.D * p.N + 2 * p.D;
-    reduce_param_kernel<<<(unsigned)((np + 255) / 256), 256, 0, s>>>(p, NP, geo.nseg * p.B, sc);
+    const int64_t bc = (p.B * p.L * p.G * 2 * p.N + 255) / 256, par = (p.D * p.N + 2 * p.D + 255) / 256;
+    if (bc + par >= ((int64_t)1 << 31)) return (int)MOGT_ERR_UNSUPPORTED;
+    reduce_kernel<T><<<(unsigned)(bc + par), 256, 0, s>>>(p, geo.nblk, NP, geo.nseg * p.B, bc, sc);
     return mogt_host::launch_status();
   });
 }

@@ -54,7 +54,8 @@ _MAX_STRIDE = 1 << 27   # the scan's kernels step over a tile's tokens with 32-b
 def _dense_last(t):
     """t itself when its last dimension is dense (and its rows are not absurdly
     far apart), else a contiguous copy."""
-    if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) <= _MAX_STRIDE):
+    if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1)
+                     and (t.stride(-2) <= _MAX_STRIDE or t.shape[-2] == 1)):
         return t
     return t.contiguous()
 
@@ -205,7 +206,7 @@ def _grouped(t, what, lead):
         t = t.unsqueeze(-2)
     if t.ndim != len(lead) + 2 or t.shape[:len(lead)] != lead:
         raise ValueError(f"{what}: B and C must be {list(lead)} + [N] or [G, N]")
-    if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-3) <= _MAX_STRIDE:
+    if (t.stride(-1) == 1 or t.shape[-1] == 1) and (t.stride(-3) <= _MAX_STRIDE or t.shape[-3] == 1):
         return t
     return t.contiguous()
 
@@ -239,20 +240,21 @@ def _check_scan(what, u, delta, A, Bm, Cm, D, z, delta_bias):
     return Bm, Cm
 
 
-def _scan_args(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus):
-    a = N.SelectiveArgs()
-    a.u, a.delta, a.z, a.Bm, a.Cm = u.data_ptr(), delta.data_ptr(), _ptr(z), Bm.data_ptr(), Cm.data_ptr()
-    a.u_sb, a.u_sl, _ = u.stride()
-    a.delta_sb, a.delta_sl, _ = delta.stride()
-    if z is not None:
-        a.z_sb, a.z_sl, _ = z.stride()
-    a.B_sb, a.B_sl, a.B_sg, _ = Bm.stride()
-    a.C_sb, a.C_sl, a.C_sg, _ = Cm.stride()
-    a.A, a.Dskip, a.bias, a.init, a.lengths = A.data_ptr(), _ptr(D), _ptr(bias), _ptr(init), _ptr(lengths)
-    a.B, a.L, a.D = u.shape
-    a.N, a.G = A.shape[1], Bm.shape[2]
-    a.softplus, a.dtype = int(softplus), _CODE[u.dtype]
-    return a
+def _token_stride(t, dim=1):
+    """A token's stride; that of a single token can be anything."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _scan_args(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus, *rest):
+    """mogt_selective_args in the order of its fields; rest: from `out` on."""
+    B, L, ch = u.shape
+    z_sb, z_sl = (0, 0) if z is None else (z.stride(0), _token_stride(z))
+    return N.SelectiveArgs(
+        u.data_ptr(), delta.data_ptr(), _ptr(z), Bm.data_ptr(), Cm.data_ptr(),
+        u.stride(0), _token_stride(u), delta.stride(0), _token_stride(delta), z_sb, z_sl,
+        Bm.stride(0), _token_stride(Bm), Bm.stride(2), Cm.stride(0), _token_stride(Cm), Cm.stride(2),
+        A.data_ptr(), _ptr(D), _ptr(bias), _ptr(init), _ptr(lengths),
+        B, L, ch, A.shape[1], Bm.shape[2], int(softplus), _CODE[u.dtype], *rest)
 
 
 def _scan_fwd(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus, return_state, save):
@@ -260,16 +262,13 @@ def _scan_fwd(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus, return_s
     n = A.shape[1]
     dev = u.device
     lib = N.lib()
-    out = torch.empty(B, L, ch, dtype=u.dtype, device=dev)
-    fin = torch.empty(B, ch, n, dtype=torch.float32, device=dev) if return_state else None
-    saved = None
-    if save:
-        saved = torch.empty(lib.mogt_selective_saved_bytes(B, L, ch, n) // 4, dtype=torch.float32, device=dev)
-    a = _scan_args(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus)
-    a.out, a.final_state, a.saved = out.data_ptr(), _ptr(fin), _ptr(saved)
-    nbytes = lib.mogt_selective_fwd_scratch_bytes(B, L, ch, n, a.G)
+    out = u.new_empty((B, L, ch))
+    fin = A.new_empty((B, ch, n)) if return_state else None
+    saved = A.new_empty(lib.mogt_selective_saved_bytes(B, L, ch, n) // 4) if save else None
+    nbytes = lib.mogt_selective_fwd_scratch_bytes(B, L, ch, n, Bm.shape[2])
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    a.scratch, a.scratch_bytes = _ptr(scratch), nbytes
+    a = _scan_args(u, delta, A, Bm, Cm, D, z, bias, init, lengths, softplus, out.data_ptr(), _ptr(fin), _ptr(saved),
+                   None, 0, 0, None, None, None, None, None, None, None, None, None, None, _ptr(scratch), nbytes)
     N.launch("mogt_selective_scan_fwd", dev, ctypes.byref(a))
     return out, fin, saved
 
@@ -306,23 +305,21 @@ class _SelectiveScanFn(torch.autograd.Function):
             dout = _dense_last(dout if dout.dtype == dt else dout.to(dt))
         dfinal = _f32(dfinal)
         Af, Df, bf = _f32(A), _f32(D), _f32(bias)
-        a = _scan_args(u, delta, Af, Bm, Cm, Df, z, bf, None, lengths, ctx.softplus)
-        vec = lambda t: None if t is None else torch.empty(ch, dtype=torch.float32, device=dev)
         du, ddelta = u.new_empty((B, L, ch)), u.new_empty((B, L, ch))
         dz = None if z is None else u.new_empty((B, L, ch))
         dB, dC = u.new_empty((B, L, G, n)), u.new_empty((B, L, G, n))
-        dA = torch.empty(ch, n, dtype=torch.float32, device=dev)
-        dD, dbias = vec(D), vec(bias)
+        dA = Af.new_empty((ch, n))
+        dD = None if D is None else Af.new_empty(ch)
+        dbias = None if bias is None else Af.new_empty(ch)
         dinit = None
         if ctx.init_dtype is not None and ctx.needs_input_grad[8]:
-            dinit = torch.empty(B, ch, n, dtype=torch.float32, device=dev)
+            dinit = Af.new_empty((B, ch, n))
         nbytes = lib.mogt_selective_bwd_scratch_bytes(B, L, ch, n, G)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a.saved, a.dout, a.dfinal = saved.data_ptr(), dout.data_ptr(), _ptr(dfinal)
-        a.dout_sb, a.dout_sl, _ = dout.stride()
-        a.du, a.ddelta, a.dz, a.dB, a.dC = du.data_ptr(), ddelta.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
-        a.dA, a.dD, a.dbias, a.dinit = dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dinit)
-        a.scratch, a.scratch_bytes = scratch.data_ptr(), nbytes
+        a = _scan_args(u, delta, Af, Bm, Cm, Df, z, bf, None, lengths, ctx.softplus, None, None, saved.data_ptr(),
+                       dout.data_ptr(), dout.stride(0), _token_stride(dout), _ptr(dfinal), du.data_ptr(),
+                       ddelta.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), _ptr(dD), _ptr(dbias),
+                       _ptr(dinit), scratch.data_ptr(), nbytes)
         with N.tag("mogt.selective_scan.backward"):
             N.launch("mogt_selective_scan_bwd", dev, ctypes.byref(a))
         cast = lambda g, t: g if g is None or t.dtype == torch.float32 else g.to(t.dtype)
