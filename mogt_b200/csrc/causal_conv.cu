@@ -71,10 +71,15 @@ __device__ __forceinline__ void narrow(Pack<T, VEC>& v, const F2 (&r)[Ch<VEC>::N
     }
   }
 }
-// 1 / (1 + e^-x) of both halves.
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// 1 / (1 + e^-x) of both halves (1 / inf = 0).
 __device__ __forceinline__ F2 sigmoid2(F2 x) {
   const float2 e = un2(add2(exp2_2(mul2(x, f2(-1.4426950408889634f, -1.4426950408889634f))), f2(1.f, 1.f)));
-  return f2(__fdividef(1.f, e.x), __fdividef(1.f, e.y));
+  return f2(rcp(e.x), rcp(e.y));
 }
 
 // The taps and bias of VEC channels.  The parameters' type is looked at once,
@@ -147,12 +152,20 @@ __global__ void __launch_bounds__(NT, kFwdCtas) fwd_kernel(const Params p) {
       widen<T, VEC>(h[j], v);
     }
     const T* x = static_cast<const T*>(p.x) + b * p.x_sb + t0 * p.x_sl + d;
+    // whole blocks step their pointers; only the last one clamps its loads and
+    // guards its stores
     Pack<T, VEC> v[UNR], next[UNR];
     auto fetch = [&](int64_t t) {
-      const int n = (int)min(te - t, (int64_t)UNR);
+      if (t + UNR <= te) {
 #pragma unroll
-      for (int r = 0; r < UNR; ++r) next[r].load(x + min(r, n - 1) * p.x_sl);
-      x += UNR * p.x_sl;
+        for (int r = 0; r < UNR; ++r) {
+          next[r].load(x);
+          x += p.x_sl;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < UNR; ++r) next[r].load(x + min((int)(te - t) - 1, r) * p.x_sl);
+      }
     };
     fetch(t0);
     for (int64_t t = t0; t < te; t += UNR) {
@@ -177,9 +190,9 @@ __global__ void __launch_bounds__(NT, kFwdCtas) fwd_kernel(const Params p) {
         }
         Pack<T, VEC> q;
         narrow<T, VEC>(q, o);
-        if (r < n) q.store(y + r * p.D);
+        if (r < n) q.store(y);
+        y += p.D;
       }
-      y += UNR * p.D;
     }
   }
   Pack<T, VEC> zero;
@@ -220,12 +233,24 @@ __global__ void __launch_bounds__(NT, kBwdCtas) bwd_kernel(const Params p) {
   }
   const int64_t first = t0 == 0 ? -(int64_t)(K - 1) : t0;  // first row emitted
   Pack<T, VEC> vx[UNR], vg[UNR], nx[UNR], ng[UNR];
-  auto fetch = [&](int64_t t) {  // tokens behind the end: the last one again
+  const T *xp = x + t0 * p.x_sl, *gp = dy + t0 * p.dy_sl;
+  T* dp = dx + (t0 - (K - 1)) * p.D;  // row of the block's first tau
+  auto fetch = [&](int64_t t) {
+    if (t + UNR <= len) {
 #pragma unroll
-    for (int r = 0; r < UNR; ++r) {
-      const int64_t tt = min(t + r, len - 1);
-      nx[r].load(x + tt * p.x_sl);
-      ng[r].load(dy + tt * p.dy_sl);
+      for (int r = 0; r < UNR; ++r) {
+        nx[r].load(xp);
+        ng[r].load(gp);
+        xp += p.x_sl;
+        gp += p.dy_sl;
+      }
+    } else {  // tokens behind the end: the last one again
+#pragma unroll
+      for (int r = 0; r < UNR; ++r) {
+        const int64_t tt = min(t + r, len - 1);
+        nx[r].load(x + tt * p.x_sl);
+        ng[r].load(dy + tt * p.dy_sl);
+      }
     }
   };
   // EDGE: tokens of the run's ends and the sequence's; inside, every token is
@@ -298,7 +323,7 @@ __global__ void __launch_bounds__(NT, kBwdCtas) bwd_kernel(const Params p) {
         }
       } else {
         narrow<T, VEC>(o, v);
-        o.store(dx + tau * p.D);
+        o.store(dp + r * p.D);
       }
     }
   };
@@ -314,6 +339,7 @@ __global__ void __launch_bounds__(NT, kBwdCtas) bwd_kernel(const Params p) {
     const bool inside = t - (K - 1) >= t0 && t + UNR <= t1 && t + UNR <= len;
     if (inside && t + UNR - K < len - (K - 1)) block(t, std::false_type{});
     else block(t, std::true_type{});
+    dp += UNR * p.D;
   }
   float* part = p.part + (b * p.runs + at.run) * (K + 1) * p.D + d;
 #pragma unroll
