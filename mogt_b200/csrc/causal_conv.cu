@@ -19,8 +19,9 @@ namespace cconv {
 
 constexpr int NT = 128;
 // CTAs on an SM and tokens a thread loads ahead, by measurement at 4 x 8192 x
-// 1536 bf16: forward 48 us with 6 and 4 (50 with 6 and 8, 57 with 5 and 8),
-// backward 88 us with 3 and 4 (96 with 4 and 4, 97 with 3 and 2, 112 with 2 and 8).
+// 1536 bf16: forward 43 us with 6 and 4 (49 with 6 and 8, 48 with 5 and 8, 51
+// with 8 and 4), backward 75 us with 3 and 4 (89 with 4 and 4, 95 with 3 and 2,
+// 74 with 3 and 6).
 constexpr int kFwdCtas = 6, kFwdUnr = 4, kBwdCtas = 3, kBwdUnr = 4;
 
 struct Params {

@@ -6,35 +6,36 @@
 //   du_t = dt_t s_t + D dy_t       ddt_t = u_t s_t + sum_n A q_t
 //   dA = sum_t dt_t q_t            dD = sum_t dy_t u_t
 //   dz_t = dout_t y_t silu'(z_t)   ddelta_t = ddt_t softplus'(delta_t + bias)
-// a_t h_{t-1} is kept as such (h_t - x_t B_t would cancel where a_t is small).
+// q_t is formed as (a_t g_t) h_{t-1}: h_t - x_t B_t would cancel where a_t is
+// small.
 //
 // The forward saved the state every 16 tokens.  A warp walks its channels'
 // tiles backwards; a tile's first 12 tokens are stepped to get the states that
-// enter its groups of 4, then each group is stepped again with a_t and
-// a_t h_{t-1} kept in registers, and walked backwards.  Lanes are those of
-// the forward (4 states each, LPC lanes per channel), and a long sequence is
+// enter its groups of 4, then each group is stepped again with a_t and h_t
+// kept in registers, and walked backwards.  Lanes are those of the forward (4
+// states of two channels each, LPC lanes per pair), and a long sequence is
 // split into segments as there, the adjoint's carries from a first pass.
 //
 // dB and dC need sums over all channels.  Per token a lane holds 8 terms (4
-// states of each), the warp's channels are added by halving exchanges that
-// leave a lane one term: a lane keeps its states in an order XORed with its
-// channel number (B and C come in as many permuted copies), so that what it
-// sends is always the same registers and no selects are needed.  The CTA's
-// warps add through shared memory and CTAs through a second kernel, in a
-// fixed order.  Instruction issue bounds it (about 20 per token, channel and
-// state), then the shuffles.
+// states of each, its two channels added), and the warp's pairs are added by
+// halving exchanges that leave a lane one term: a lane keeps its states in an
+// order XORed with its pair's number (B and C come in as many permuted
+// copies), so that what it sends is always the same registers and no selects
+// are needed.  The CTA's warps add through shared memory and CTAs through a
+// second kernel, in a fixed order.
+//
+// 8192 x 1536 x 16 bf16: 320 us, with the first pass 402.  Bound by
+// shared-memory wavefronts (62 % of their peak) together with instruction
+// issue (54 %); HBM is at 8 %.
 #include "selective_scan.cuh"
 
 namespace mogt {
 namespace sel {
 
-#ifndef MOGT_BWD_WARPS
-#define MOGT_BWD_WARPS 16
-#endif
 // CTAs on an SM by registers and shared memory.  For 4 lanes per pair (N = 16)
-// three of 168 registers: 355 us at 8192 x 1536 (before operands were copied
-// asynchronously, 320 us since), against 427 us for two of 255
-// and 439 us for four of 128, which spill.
+// three of 168 registers: 355 us at 8192 x 1536 (320 us since operands are
+// copied asynchronously), against 427 us for two of 255 and 439 us for four of
+// 128, which spill.
 constexpr int bwd_ctas(int lpc) { return lpc == 4 ? 3 : lpc == 1 ? 1 : 2; }
 // The first pass over a split sequence costs about a quarter of the main one.
 inline int64_t bwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {

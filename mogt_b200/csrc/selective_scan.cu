@@ -23,8 +23,8 @@
 namespace mogt {
 namespace sel {
 
-// The first pass costs about 0.7 of the main one (320 against 410 us at 32768 x
-// 1536, N = 16).
+// The first pass costs about 0.75 of the main one (267 against 349 us at 32768 x
+// 1536, N = 16; it takes one segment less).
 inline int64_t fwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {
   return num_segments(B, L, D, N, G, NT, 148 * fwd_ctas(lpc_of(N)), 0.7f);
 }
