@@ -171,15 +171,14 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
 
     with lp = log softmax(logits)[label], r = exp(lp - old_logprobs),
     d = ref_logprobs - lp and a the advantage.  old_logprobs, ref_logprobs:
-    [B, L] (the KL term needs ref_logprobs); advantages: [B] or [B, L].
+    [B, L] (without ref_logprobs there is no KL term, whatever kl_coef is);
+    advantages: [B] or [B, L].
     Returns the loss (fp32 scalar), with ``return_logprobs`` also lp [B, L]."""
     what = "policy_loss"
     _cuda(what, logits, labels, old_logprobs, advantages, ref_logprobs, mask)
     logits, labels, mask = _rows(what, logits, labels, mask)
     shape = labels.shape
     old = _token_f32(what, "old_logprobs", old_logprobs, shape)
-    if kl_coef != 0.0 and ref_logprobs is None:
-        raise ValueError(f"{what}: kl_coef needs ref_logprobs")
     ref = None if ref_logprobs is None else _token_f32(what, "ref_logprobs", ref_logprobs, shape)
     if advantages.shape not in (shape, shape[:1]):
         raise ValueError(f"{what}: advantages must be [B] or [B, L]")

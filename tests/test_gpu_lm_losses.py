@@ -227,6 +227,14 @@ def test_gradient_against_differences():
     assert abs(num - ana) <= 1e-2 * abs(ana)
 
 
+def test_no_kl_term_without_reference():
+    import mogt_b200
+    t = make(2, 5, 60, F32)
+    args = (t["logits"], t["labels"], t["old"], t["adv"])
+    assert torch.equal(mogt_b200.policy_loss(*args, mask=t["mask"], kl_coef=0.3),
+                       mogt_b200.policy_loss(*args, mask=t["mask"]))
+
+
 def test_refusals():
     import mogt_b200
     x, lab = torch.zeros(2, 3, 10, device="cuda"), torch.zeros(2, 3, dtype=torch.int64, device="cuda")
@@ -242,7 +250,6 @@ def test_refusals():
             ("CUDA", lambda: mogt_b200.token_logprobs(x, lab.cpu())),
             ("old_logprobs", lambda: mogt_b200.policy_loss(x, lab, p, p)),
             ("advantages", lambda: mogt_b200.policy_loss(x, lab, f, f[:, :2])),
-            ("ref_logprobs", lambda: mogt_b200.policy_loss(x, lab, f, p, kl_coef=0.1)),
             ("ref_logprobs", lambda: mogt_b200.policy_loss(x, lab, f, p, ref_logprobs=p, kl_coef=0.1)),
             ("clip", lambda: mogt_b200.policy_loss(x, lab, f, p, clip_low=-0.1)),
             ("preferred", lambda: mogt_b200.preference_loss(x[:1], lab[:1], p[:1])),
