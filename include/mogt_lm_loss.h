@@ -31,11 +31,12 @@ int mogt_logprob_fwd(const void* logits, int64_t sb, int64_t sl, const int64_t* 
                      const uint8_t* mask, int64_t B, int64_t L, int64_t V, int dtype,
                      float* logprobs, float* stats, void* stream);
 /* dlogits[r] = coef[r / coef_div] * (onehot(label) - softmax(logits[r])),
- * coef f32, times *scale when scale is not NULL. */
+ * coef f32, times *scale when scale is not NULL.  unless_one: leave dlogits as
+ * it is when *scale is 1 (read on the device). */
 int mogt_logprob_bwd(const void* logits, int64_t sb, int64_t sl, const int64_t* labels,
                      const uint8_t* mask, const float* stats, const float* coef, int64_t coef_div,
-                     const float* scale, void* dlogits, int64_t d_sb, int64_t d_sl, int64_t B,
-                     int64_t L, int64_t V, int dtype, void* stream);
+                     const float* scale, int unless_one, void* dlogits, int64_t d_sb,
+                     int64_t d_sl, int64_t B, int64_t L, int64_t V, int dtype, void* stream);
 
 /* Clipped policy loss over the n counting tokens, lp = their log-probability,
  * r = exp(lp - old), d = ref - lp:
@@ -61,10 +62,6 @@ int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, const int64_t* 
  * mogt_logprob_bwd with coef_div = L. */
 int mogt_preference_pairs(const float* logprobs, const float* ref, int64_t P, int64_t L, float beta,
                           float eps, float* loss, float* seq, float* coef, void* stream);
-
-/* x *= *scale for a dense array; returns without touching it when *scale is
- * 1 (read on the device). */
-int mogt_scale_unless_one(void* x, int64_t n, int dtype, const float* scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -84,13 +84,12 @@ SIGNATURES = {
     "mogt_selective_step": (_int, [_vp, _vp] + [_vp, _i64] * 3 + [_vp, _i64, _i64] * 2 + [_vp] * 4 + [_i64] * 4
                             + [_int, _int, _vp]),
     "mogt_logprob_fwd": (_int, [_vp, _i64, _i64, _vp, _vp] + [_i64] * 3 + [_int] + [_vp] * 3),
-    "mogt_logprob_bwd": (_int, [_vp, _i64, _i64] + [_vp] * 4 + [_i64, _vp, _vp, _i64, _i64] + [_i64] * 3
+    "mogt_logprob_bwd": (_int, [_vp, _i64, _i64] + [_vp] * 4 + [_i64, _vp, _int, _vp, _i64, _i64] + [_i64] * 3
                          + [_int, _vp]),
     "mogt_policy_loss_scratch_bytes": (_sz, [_i64] * 2),
     "mogt_policy_loss": (_int, [_vp, _i64, _i64] + [_vp] * 5 + [_i64, _i64] + [_f32] * 3 + [_vp] * 5
                          + [_i64, _i64] + [_i64] * 3 + [_int, _vp, _sz, _vp]),
     "mogt_preference_pairs": (_int, [_vp, _vp, _i64, _i64, _f32, _f32] + [_vp] * 4),
-    "mogt_scale_unless_one": (_int, [_vp, _i64, _int, _vp, _vp]),
 }
 
 _lib = None

@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(NT, Tune<NT>::kCtas) rows_kernel(const Rows r,
 
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT, Tune<NT>::kCtas) rows_bwd_kernel(const Rows r, const float* coef, int64_t coef_div,
-                                                      const float* scale) {
+                                                      const float* scale, bool unless_one) {
+  if (unless_one && *scale == 1.f) return;
   const int64_t row = blockIdx.x;
   const int64_t b = row / r.L, l = row % r.L;
   T* d = static_cast<T*>(r.d) + b * r.d_sb + l * r.d_sl;
@@ -348,14 +349,6 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const float* lp, const floa
   if (threadIdx.x == 0) *loss = (float)(tot / (double)(P > 0 ? P : 1));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) scale_kernel(T* x, int64_t n, const float* scale) {
-  const float s = *scale;
-  if (s == 1.f) return;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-    x[i] = from_f32<T>(s * to_f32(x[i]));
-}
-
 template <typename F>
 int by_type(int dtype, F&& f) {
   switch (dtype) {
@@ -402,18 +395,20 @@ extern "C" int mogt_logprob_fwd(const void* logits, int64_t sb, int64_t sl, cons
 
 extern "C" int mogt_logprob_bwd(const void* logits, int64_t sb, int64_t sl, const int64_t* labels,
                                 const uint8_t* mask, const float* stats, const float* coef, int64_t coef_div,
-                                const float* scale, void* dlogits, int64_t d_sb, int64_t d_sl, int64_t B, int64_t L,
+                                const float* scale, int unless_one, void* dlogits, int64_t d_sb, int64_t d_sl,
+                                int64_t B, int64_t L,
                                 int64_t V, int dtype, void* stream) {
   if (int st = check(B, L, V, dtype)) return st;
   if (coef_div <= 0) return MOGT_ERR_SHAPE;
   if (B * L == 0) return MOGT_OK;
-  if (!logits || !labels || !stats || !coef || !dlogits) return MOGT_ERR_ARG;
+  if (!logits || !labels || !stats || !coef || !dlogits || (unless_one && !scale)) return MOGT_ERR_ARG;
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, nullptr,
          const_cast<float2*>(reinterpret_cast<const float2*>(stats))};
   return by_type(dtype, [&](auto t) {
     return by_rows<256>(r.rows, [&](auto n) {
       constexpr int NT = decltype(n)::value;
-      rows_bwd_kernel<decltype(t), NT><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(r, coef, coef_div, scale);
+      rows_bwd_kernel<decltype(t), NT><<<(unsigned)r.rows, NT, 0, (cudaStream_t)stream>>>(
+          r, coef, coef_div, scale, unless_one != 0);
       return mogt_host::launch_status();
     });
   });
@@ -463,17 +458,4 @@ extern "C" int mogt_preference_pairs(const float* logprobs, const float* ref, in
   if (!loss || (P > 0 && (!ref || !seq || !coef || (L > 0 && !logprobs)))) return MOGT_ERR_ARG;
   pairs_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(logprobs, ref, P, L, beta, eps, loss, seq, coef);
   return mogt_host::launch_status();
-}
-
-extern "C" int mogt_scale_unless_one(void* x, int64_t n, int dtype, const float* scale, void* stream) {
-  if (n < 0) return MOGT_ERR_SHAPE;
-  if (n == 0) return MOGT_OK;
-  if (!x || !scale) return MOGT_ERR_ARG;
-  const int64_t blocks = (n + 1023) / 1024;
-  return by_type(dtype, [&](auto t) {
-    using T = decltype(t);
-    scale_kernel<T><<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), 256, 0, (cudaStream_t)stream>>>(
-        static_cast<T*>(x), n, scale);
-    return mogt_host::launch_status();
-  });
 }

@@ -61,14 +61,16 @@ def _logprob_fwd(logits, labels, mask, want_stats):
     return lp, stats
 
 
-def _logprob_bwd(logits, labels, mask, stats, coef, coef_div, scale):
-    """stats, coef: addresses of f32 [B, L, 2] and [B * L / coef_div]."""
+def _logprob_bwd(logits, labels, mask, stats, coef, coef_div, scale, d=None):
+    """stats, coef: addresses of f32 [B, L, 2] and [B * L / coef_div].  d: a
+    gradient that is right already if scale is 1; a new one otherwise."""
     B, L, V = logits.shape
     dev = logits.device
-    d = _grad_like(logits)
+    unless_one = d is not None
+    d = d if unless_one else _grad_like(logits)
     scale = _f32(scale)
     N.launch("mogt_logprob_bwd", dev, logits.data_ptr(), logits.stride(0), logits.stride(1), labels.data_ptr(),
-             _ptr(mask), stats, coef, coef_div, _ptr(scale), d.data_ptr(), d.stride(0), d.stride(1), B, L, V,
+             _ptr(mask), stats, coef, coef_div, _ptr(scale), unless_one, d.data_ptr(), d.stride(0), d.stride(1), B, L, V,
              _CODE[logits.dtype])
     return d
 
@@ -123,10 +125,11 @@ def _policy(logits, labels, mask, old, ref, adv, lo, hi, kl, want_grad):
 
 class _PolicyLossFn(torch.autograd.Function):
     """The forward also writes the gradient for d loss = 1 (the rows are on the
-    chip at that moment); the backward hands it out, scaled in place unless
-    the incoming gradient is 1.  A second backward (retain_graph) forms it
-    again from the logits, since the first one may have been changed by its
-    receiver."""
+    chip at that moment) and the backward hands it out.  For another incoming
+    gradient (a scaled loss) it is formed again from the logits, so that it is
+    rounded once, with the scale: an fp16 gradient scaled afterwards would have
+    lost what the scale is there to save.  So is that of a second backward
+    (retain_graph), since the first one may have been changed by its receiver."""
 
     @staticmethod
     def forward(ctx, logits, labels, mask, old, ref, adv, lo, hi, kl):
@@ -144,16 +147,10 @@ class _PolicyLossFn(torch.autograd.Function):
         if g is None:
             return (None,) * 9
         d, ctx.grad = ctx.grad, None
+        logits, labels, mask, work = ctx.saved_tensors
+        at = work.data_ptr()
         with N.tag("mogt.policy_loss.backward"):
-            if d is None:
-                logits, labels, mask, work = ctx.saved_tensors
-                at = work.data_ptr()
-                d = _logprob_bwd(logits, labels, mask, at, at + 8 * labels.numel(), 1, g)
-            else:
-                base = d if d.is_contiguous() else d._base
-                g = _f32(g)
-                N.launch("mogt_scale_unless_one", d.device, base.data_ptr(), base.numel(), _CODE[d.dtype],
-                         g.data_ptr())
+            d = _logprob_bwd(logits, labels, mask, at, at + 8 * labels.numel(), 1, g, d)
         return d, None, None, None, None, None, None, None, None
 
 

@@ -173,6 +173,22 @@ def test_scaled_and_repeated_backward():
     assert max_err(x.grad, 2.0 * g64) <= TOL32
 
 
+@pytest.mark.parametrize("dtype,scale", [(F16, 65536.0), (BF16, 1.0 / 3.0), (F16, 1.0), (BF16, 1.0)])
+def test_a_scaled_loss_is_rounded_once(dtype, scale):
+    """Gradients of a mean over many tokens are below fp16's smallest number
+    before a loss scale brings them up: the scale goes in before the rounding."""
+    t = make(4, 64, 500, dtype, pad=4)
+    x, loss, _, x64, loss64, _ = policy(t, dtype)
+    g, = torch.autograd.grad(loss * scale, x)
+    g64, = torch.autograd.grad(loss64 * scale, x64)
+    floor = 2.0 ** -25 / float(g64.abs().max()) if dtype == F16 else 0.0
+    assert max_err(g, g64) <= TOL32 + ROUND[dtype] + floor
+    big = g64.abs() > 2.0 ** -14          # normal numbers of either type: one rounding each
+    err = (g.double() - g64).abs()[big] / g64.abs()[big]
+    # beyond the rounding: p carries the fp32 error of its exponential and, as 1 - p at the label, a cancellation
+    assert float(err.max()) <= ROUND[dtype] + 2.0 ** -16
+
+
 def test_per_token_advantages_and_views():
     t = make(4, 6, 200, F32)
     adv = torch.randn(4, 12, device="cuda")[:, ::2]

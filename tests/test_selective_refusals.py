@@ -57,7 +57,9 @@ def test_c_abi_checks_its_arguments():
     assert lib.mogt_policy_loss(p, 0, 0, p, None, p, None, p, 0, 0, 0.2, 0.2, 0.0, p, p, None, p, None, 0, 0, 1, 1, 5, 0,
                                 None, 0, None) == N.ERR_WORKSPACE
     assert lib.mogt_preference_pairs(p, None, 1, 1, 0.1, 0.0, p, p, p, None) == N.ERR_ARG
-    assert lib.mogt_scale_unless_one(None, 4, 0, p, None) == N.ERR_ARG
+    bwd = lambda scale, unless: lib.mogt_logprob_bwd(p, 0, 0, p, None, p, p, 1, scale, unless, None, 0, 0, 1, 1, 5, 0,
+                                                    None)
+    assert bwd(p, 0) == N.ERR_ARG and bwd(None, 1) == N.ERR_ARG
 
 
 def test_scratch_sizes():
