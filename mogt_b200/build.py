@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -38,22 +39,23 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     sources = sorted(CSRC.glob("*.cu"))
     headers = sorted(CSRC.glob("*.cuh")) + sorted((PKG.parent / "include").glob("*.h"))
     newest_hdr = max((h.stat().st_mtime for h in headers), default=0.0)
-    objs = []
-    for src in sources:
-        obj = BUILD / (src.stem + ".o")
-        objs.append(obj)
-        if (not force and obj.exists() and obj.stat().st_mtime >= src.stat().st_mtime
-                and obj.stat().st_mtime >= newest_hdr):
-            continue
-        cmd = [nvcc(), *ARCH, *FLAGS, "-c", str(src), "-o", str(obj)]
-        res = subprocess.run(cmd, capture_output=True, text=True)
-        log = BUILD / (src.stem + ".ptxas.txt")
-        log.write_text(res.stdout + res.stderr)
-        if res.returncode != 0:
-            sys.stderr.write(res.stdout + res.stderr)
-            raise RuntimeError(f"nvcc failed on {src.name}")
-        if verbose:
-            sys.stdout.write(res.stderr)
+    objs = [BUILD / (src.stem + ".o") for src in sources]
+    stale = [(src, obj) for src, obj in zip(sources, objs)
+             if force or not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, newest_hdr)]
+
+    def compile_one(job):
+        src, obj = job
+        res = subprocess.run([nvcc(), *ARCH, *FLAGS, "-c", str(src), "-o", str(obj)], capture_output=True, text=True)
+        (BUILD / (src.stem + ".ptxas.txt")).write_text(res.stdout + res.stderr)
+        return src, res
+
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        for src, res in pool.map(compile_one, stale):
+            if res.returncode != 0:
+                sys.stderr.write(res.stdout + res.stderr)
+                raise RuntimeError(f"nvcc failed on {src.name}")
+            if verbose:
+                sys.stdout.write(res.stderr)
     if force or not LIB.exists() or any(o.stat().st_mtime > LIB.stat().st_mtime for o in objs):
         cmd = [nvcc(), *ARCH, "-shared", "-o", str(LIB), *map(str, objs), "-cudart", "static"]
         res = subprocess.run(cmd, capture_output=True, text=True)
