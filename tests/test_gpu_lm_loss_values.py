@@ -1,0 +1,30 @@
+"""Post-training losses where their values are delicate: sums of thousands that
+nearly cancel, terms without weight, logits that are slices of larger tensors."""
+import pytest
+import torch
+
+from .selective_ref import ROUND, max_err, preference_ref
+from .test_gpu_lm_losses import TOL32, make, policy
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_preference_of_long_responses(seed):
+    """Two sums of about -4000 whose difference is a few tens.  A token's
+    log-probability is off by at most 2^-19 (a difference of values below 16
+    and a logarithm below 16, each rounded to 24 bits), independently from
+    token to token: over the 2 L tokens of a pair sqrt(2 L) 2^-19, times beta,
+    and the loss moves by no more than its logit does.  Sums kept in 32 bits
+    would be off by 2^-13 each before anything else."""
+    import mogt_b200
+    B, L, V, beta = 8, 512, 32001, 0.1
+    t = make(B, L, V, BF16, seed=seed)
+    ref = (t["sref"] + 5 * torch.randn(B, generator=torch.Generator("cuda").manual_seed(seed), device="cuda"))
+    loss, seq = mogt_b200.preference_loss(t["logits"], t["labels"], ref, beta=beta, label_smoothing=0.05,
+                                          mask=t["mask"], return_logprobs=True)
+    loss64, seq64 = preference_ref(t["logits"].double(), t["labels"], t["counts"], ref.double(), beta, 0.05)
+    assert abs(float(loss) - float(loss64)) <= (2 * L) ** 0.5 * 2.0 ** -19 * beta
+    assert max_err(seq, seq64) <= TOL32
