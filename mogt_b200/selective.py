@@ -22,7 +22,10 @@ state after the sequence's last token.
 
 The prompt forms are differentiable in every floating tensor, the states
 included.  The single-token forms are for generation: they record no gradient
-and update the state in place, or into ``new_state``.
+and update the state in place, or into ``new_state``.  What they write counts
+as modified in place: a recorded call that still needs it raises in its
+backward, and a state that itself requires grad is not written while gradients
+are recorded.
 """
 from __future__ import annotations
 
@@ -79,6 +82,18 @@ def _f32(t):
     if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
         return t
     return t.to(torch.float32).contiguous()
+
+
+def _writable(what, new_state):
+    if new_state.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{what}: the state to write requires grad, and the call records none: "
+                         "detach it, or call under torch.no_grad()")
+
+
+def _written(new_state):
+    """The kernels write through a pointer; autograd sees it by the version."""
+    if not new_state.is_inference():
+        torch.autograd.graph.increment_version(new_state)
 
 
 def _activation(activation):
@@ -190,10 +205,12 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
     for s in (state, new_state):
         if s.shape != (B, K - 1, D) or s.dtype != x.dtype or not s.is_contiguous():
             raise ValueError(f"{what}: state must be a contiguous [B, K-1, D] in x's dtype")
+    _writable(what, new_state)
     x = _dense_last(x)
     y = torch.empty(B, D, dtype=x.dtype, device=dev)
     N.launch("mogt_causal_conv_step", dev, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _ptr(bias),
              y.data_ptr(), new_state.data_ptr(), B, D, K, silu, _CODE[x.dtype], _CODE[weight.dtype])
+    _written(new_state)
     return y
 
 
@@ -374,6 +391,7 @@ def selective_scan_step(state, u, delta, A, B, C, *, D=None, z=None, delta_bias=
     for s in (state, new_state):
         if s.shape != (bs, ch, n) or s.dtype != torch.float32 or not s.is_contiguous():
             raise ValueError(f"{what}: state must be a contiguous [B, D, N] float32")
+    _writable(what, new_state)
     u, delta, z = _dense_last(u), _dense_last(delta), _dense_last(z)
     A, D, delta_bias = _f32(A), _f32(D), _f32(delta_bias)
     y = torch.empty(bs, ch, dtype=u.dtype, device=dev)
@@ -383,4 +401,5 @@ def selective_scan_step(state, u, delta, A, B, C, *, D=None, z=None, delta_bias=
              delta.data_ptr(), delta.stride(0), _ptr(z), 0 if z is None else z.stride(0), Bm.data_ptr(), b_sb, b_sg,
              Cm.data_ptr(), c_sb, c_sg, A.data_ptr(), _ptr(D), _ptr(delta_bias), y.data_ptr(), bs, ch, n, Bm.shape[1],
              int(delta_softplus), _CODE[u.dtype])
+    _written(new_state)
     return y
