@@ -106,15 +106,23 @@ class SelectiveLM(nn.Module):
 
     @torch.no_grad()
     def prefill(self, input_ids, lengths=None):
-        """Logits after each prompt's last token [B, vocab], and the caches."""
+        """Logits after each prompt's last token [B, vocab], and the caches.
+        lengths are clamped to [0, L] as in the operators; a prompt without
+        tokens has all logits 0."""
         B, L = input_ids.shape
         x = self.embedding(input_ids)
         caches = []
         for blk in self.blocks:
             x, cache = blk.prefill(x, lengths)
             caches.append(cache)
-        last = torch.full((B,), L, device=x.device) if lengths is None else lengths
-        x = x[torch.arange(B, device=x.device), last.long() - 1]
+        if L == 0:
+            x = x.new_zeros(B, x.shape[-1])
+        elif lengths is None:
+            x = x[:, -1]
+        else:
+            n = lengths.long().clamp(0, L)
+            x = x[torch.arange(B, device=x.device), (n - 1).clamp(min=0)]
+            x = torch.where((n > 0)[:, None], x, 0.0)
         return self._head(x), caches
 
     @torch.no_grad()
