@@ -360,7 +360,8 @@ extern "C" int mogt_selective_step(const float* state, float* new_state, const v
   const uintptr_t bcs = reinterpret_cast<uintptr_t>(Bm) | reinterpret_cast<uintptr_t>(Cm);
   const bool v4 = N % 4 == 0 && f32s % 16 == 0 && bcs % (dtype == MOGT_DTYPE_F32 ? 16 : 8) == 0 &&
                   (B_sb | B_sg | C_sb | C_sg) % 4 == 0;
-  if (D > kMaxStride) return MOGT_ERR_UNSUPPORTED;
+  // channels and their threads are counted in 32 bits
+  if (D > kMaxStride || D * lpc_of(N) > INT32_MAX - NT) return MOGT_ERR_UNSUPPORTED;
   StepParams p{};
   p.state = state; p.new_state = new_state;
   p.u = u; p.delta = delta; p.z = z; p.Bm = Bm; p.Cm = Cm;
