@@ -24,8 +24,10 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Seven terms leave 1.5e-8; relative accuracy for small e, which the step
 // sizes near softplus' lower end need, comes with the series.  The exponent's
 // rounding error is put back (a product rounded at |x| = 10 is off by 5e-7).
+// |x| is cut off where e is 0 in any case: a delta of -inf or of the type's
+// lowest value masks a step, and inf - inf must not be formed from it.
 __device__ __forceinline__ float exp_neg_abs(float x) {
-  const float a = -fabsf(x), t = a * kLog2e;
+  const float a = -fminf(fabsf(x), 127.f), t = a * kLog2e;
   return fast_exp2(t) * fmaf(fmaf(a, kLog2e, -t), kLn2, 1.f);
 }
 __device__ __forceinline__ float softplus_e(float x, float e) {
