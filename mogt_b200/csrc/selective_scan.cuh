@@ -1,6 +1,7 @@
 // Lane layout, tiles and dispatch shared by the selective scan's forward and backward.
 #pragma once
 
+#include <cfloat>
 #include <initializer_list>
 #include <type_traits>
 
@@ -238,6 +239,22 @@ struct SegScratch {
   float* sdt;   // [nseg - 1][B][D]
 };
 
+// exp(dt A) x where exp(dt A) alone is beyond the largest float (growing
+// states: A or dt of the other sign): nothing stays nothing, and by the square
+// root twice a small x gets the value that it grows to.
+__device__ __forceinline__ float grown(float dt, float A2, float x) {
+  const float r = fast_exp2(0.5f * fmaf(dt, A2, kExp2Shift));
+  return x == 0.f ? 0.f : x * r * r;
+}
+// a x + l for both halves, a = exp(sd A) over a whole segment.
+__device__ __forceinline__ F2 carry(F2 sd, F2 A2, F2 x, F2 l) {
+  const F2 a = decay(sd, A2);
+  const float2 v = un2(a);
+  if (!(fmaxf(v.x, v.y) > FLT_MAX)) return fma2(a, x, l);
+  const float2 d = un2(sd), e = un2(A2), s = un2(x);
+  return add2(f2(v.x > FLT_MAX ? grown(d.x, e.x, s.x) : v.x * s.x, v.y > FLT_MAX ? grown(d.y, e.y, s.y) : v.y * s.y), l);
+}
+
 // The state (or adjoint) entering a segment: the chain over segments
 // first, first + step, ..., count of them.  x: what the chain starts from.
 template <int LPC, typename W, bool PERM>
@@ -252,10 +269,10 @@ __device__ __forceinline__ void chain(F2 (&x)[NS], const F2 (&A2)[NS], const Seg
       l1 = Perm<LPC>::apply(l1, w.c);
     }
     const F2 sd = f2(s.sdt[i], s.sdt[i + w.ok1]);
-    x[0] = fma2(decay(sd, A2[0]), x[0], f2(l0.x, l1.x));
-    x[1] = fma2(decay(sd, A2[1]), x[1], f2(l0.y, l1.y));
-    x[2] = fma2(decay(sd, A2[2]), x[2], f2(l0.z, l1.z));
-    x[3] = fma2(decay(sd, A2[3]), x[3], f2(l0.w, l1.w));
+    x[0] = carry(sd, A2[0], x[0], f2(l0.x, l1.x));
+    x[1] = carry(sd, A2[1], x[1], f2(l0.y, l1.y));
+    x[2] = carry(sd, A2[2], x[2], f2(l0.z, l1.z));
+    x[3] = carry(sd, A2[3], x[3], f2(l0.w, l1.w));
   }
 }
 

@@ -48,3 +48,38 @@ def test_a_step_as_large_as_the_type_allows():
     y, h = mogt_b200.selective_scan(one * 2.0 ** -20, one * big, -one[0], one, one, delta_softplus=True,
                                     return_state=True)
     assert float(y) == float(h) == big * 2.0 ** -20
+
+
+def _growing(L, G=1):
+    """exp(dt A) = e^2 a token: over a segment of 64 tokens or more the decay alone overflows."""
+    t = make(1, L, 8, 4, G, F32, z=False, skip=False, bias=False)
+    t["A"] = torch.full_like(t["A"], 2.0)
+    t["delta"] = torch.ones_like(t["delta"])
+    return t
+
+
+def test_growing_states_start_from_nothing():
+    """Zero inputs up to the last 20 tokens, and gradients of the first 20
+    outputs only: all values are far from the largest, on either way."""
+    t = _growing(4096)
+    t["u"][:, :-20] = 0
+    t["dout"][:, 20:] = 0
+    t["dfinal"] = torch.zeros_like(t["dfinal"])
+    compare(run(t, softplus=False), ref(t, softplus=False), 20)
+
+
+def test_growing_states_that_fit():
+    """A state of 1e-30 that grows by e^128 over a segment, and stays below
+    3e38.  The exponents' rounding (2^-17 of exponents up to 256) is all of the
+    error beyond the steps'."""
+    import mogt_b200
+    L = 4040
+    t = _growing(4096)
+    t["u"][:] = 0
+    t["u"][:, 3967] = 1e-30
+    lengths = torch.tensor([L], device="cuda")
+    args = [t[k] for k in ("u", "delta", "A", "B", "C")]
+    y, h = mogt_b200.selective_scan(*args, lengths=lengths, return_state=True)
+    assert bool(torch.isfinite(y).all()) and bool(torch.isfinite(h).all())
+    y64, h64 = scan_ref(*[a.double() for a in args], softplus=False, lengths=lengths)
+    assert max_err(y, y64) <= 2.0 ** -15 and max_err(h, h64) <= 2.0 ** -15
