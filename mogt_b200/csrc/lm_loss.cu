@@ -430,8 +430,9 @@ extern "C" int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, cons
   if (!scratch || scratch_bytes < mogt_policy_loss_scratch_bytes(B, L)) return MOGT_ERR_WORKSPACE;
   float* inv_n = static_cast<float*>(scratch);
   Rows r{logits, sb, sl, labels, mask, L, V, B * L, dlogits, d_sb, d_sl, logprobs, reinterpret_cast<float2*>(stats)};
-  Policy q{old_logprobs, ref_logprobs, adv, adv_sb, adv_sl, 1.f - clip_low, 1.f + clip_high, kl_coef, inv_n,
-           r.rows > kInlineCount || r.rows == 0, inv_n + 1, coef};
+  // a weight of 0 is no term: exp(ref - lp) may overflow, and 0 * inf is not 0
+  Policy q{old_logprobs, kl_coef != 0.f ? ref_logprobs : nullptr, adv, adv_sb, adv_sl, 1.f - clip_low, 1.f + clip_high,
+           kl_coef, inv_n, r.rows > kInlineCount || r.rows == 0, inv_n + 1, coef};
   cudaStream_t s = (cudaStream_t)stream;
   return by_type(dtype, [&](auto t) {
     using T = decltype(t);

@@ -28,3 +28,19 @@ def test_preference_of_long_responses(seed):
     loss64, seq64 = preference_ref(t["logits"].double(), t["labels"], t["counts"], ref.double(), beta, 0.05)
     assert abs(float(loss) - float(loss64)) <= (2 * L) ** 0.5 * 2.0 ** -19 * beta
     assert max_err(seq, seq64) <= TOL32
+
+
+def test_no_kl_weight_is_no_kl_term():
+    """exp(ref - lp) overflows for a label that the model all but excludes; with kl_coef = 0 that is no term at all."""
+    import mogt_b200
+    x = torch.zeros(1, 3, 10, device="cuda")
+    x[0, 1, 4] = -200.0
+    lab = torch.full((1, 3), 4, device="cuda")
+    lp = mogt_b200.token_logprobs(x, lab)
+    adv = torch.ones(1, device="cuda")
+    a = x.clone().requires_grad_(True)
+    b = x.clone().requires_grad_(True)
+    la = mogt_b200.policy_loss(a, lab, lp, adv, ref_logprobs=torch.zeros_like(lp))
+    lb = mogt_b200.policy_loss(b, lab, lp, adv)
+    assert torch.equal(la, lb) and float(lb.detach()) == -1.0
+    assert torch.equal(torch.autograd.grad(la, a)[0], torch.autograd.grad(lb, b)[0])
