@@ -337,7 +337,8 @@ __global__ void __launch_bounds__(1024) pairs_kernel(const float* lp, const floa
     }
     if (lane == 0) {
       const float x = (float)((double)beta * ((s[0] - (double)ref[i]) - (s[1] - (double)ref[P + i])));
-      tot -= (1.f - eps) * log_sigmoid(x) + eps * log_sigmoid(-x);
+      // a side without weight is no term: x is infinite for a response of probability 0
+      tot -= (eps < 1.f ? (1.f - eps) * log_sigmoid(x) : 0.f) + (eps > 0.f ? eps * log_sigmoid(-x) : 0.f);
       const float c = beta / (float)P * (eps / (1.f + expf(-x)) - (1.f - eps) / (1.f + expf(x)));
       seq[i] = (float)s[0];
       seq[P + i] = (float)s[1];

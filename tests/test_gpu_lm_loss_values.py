@@ -44,3 +44,23 @@ def test_no_kl_weight_is_no_kl_term():
     lb = mogt_b200.policy_loss(b, lab, lp, adv)
     assert torch.equal(la, lb) and float(lb.detach()) == -1.0
     assert torch.equal(torch.autograd.grad(la, a)[0], torch.autograd.grad(lb, b)[0])
+
+
+def test_an_impossible_response_of_a_pair():
+    """A response with a label at -inf has probability zero: rejected, its pair
+    is settled (x = inf, loss 0 without smoothing); preferred, its loss is inf,
+    and 0 where the smoothing of 1 swaps the pair."""
+    import mogt_b200
+    lab = torch.full((2, 3), 4, device="cuda")
+    ref = torch.zeros(2, device="cuda")
+    for rejected, eps, want in ((True, 0.0, 0.0), (False, 1.0, 0.0), (False, 0.0, float("inf")),
+                                (True, 0.25, float("inf"))):
+        x = torch.randn(2, 3, 10, device="cuda")
+        x[int(rejected), 1, 4] = float("-inf")
+        x.requires_grad_(True)
+        loss = mogt_b200.preference_loss(x, lab, ref, label_smoothing=eps)
+        assert float(loss.detach()) == want, (rejected, eps, float(loss.detach()))
+        g, = torch.autograd.grad(loss, x)
+        assert bool(torch.isfinite(g).all())
+        if want == 0.0:
+            assert bool((g == 0).all())
