@@ -43,12 +43,19 @@ def _rows(what, logits, labels, mask):
 
 def _grad_like(logits):
     """An empty [B, L, V] whose rows start at the same offsets from a 16-byte
-    boundary as those of logits, so that both are accessed 16 bytes at a time."""
+    boundary as those of logits (slices of a wider head or of the tokens
+    included), so that both are accessed 16 bytes at a time; rows are as close
+    together as that allows."""
     B, L, V = logits.shape
     sb, sl, _ = logits.stride()
-    if sl >= V and sb == L * sl and logits.data_ptr() % 16 == 0:
-        return torch.empty(B, L, sl, dtype=logits.dtype, device=logits.device)[..., :V]
-    return torch.empty(B, L, V, dtype=logits.dtype, device=logits.device)
+    e = logits.element_size()
+    first = logits.data_ptr() % 16 // e
+    row = V + (sl - V) % (16 // e) if L > 1 else V
+    batch = L * row + (sb - L * row) % (16 // e) if B > 1 else L * row
+    if first == 0 and row == V and batch == L * V:
+        return torch.empty(B, L, V, dtype=logits.dtype, device=logits.device)
+    room = torch.empty(first + B * batch, dtype=logits.dtype, device=logits.device)
+    return room.as_strided((B, L, V), (batch, row, 1), first)
 
 
 def _logprob_fwd(logits, labels, mask, want_stats):

@@ -64,3 +64,43 @@ def test_an_impossible_response_of_a_pair():
         assert bool(torch.isfinite(g).all())
         if want == 0.0:
             assert bool((g == 0).all())
+
+
+def _address(t):
+    """Offsets from a 16-byte boundary of every row."""
+    e = t.element_size()
+    at = torch.arange(t.shape[0])[:, None] * t.stride(0) + torch.arange(t.shape[1])[None] * t.stride(1)
+    return (t.data_ptr() + at * e) % 16
+
+
+@pytest.mark.parametrize("dtype,V", [(BF16, 1001), (F32, 1001), (F16, 515), (BF16, 1024)])
+@pytest.mark.parametrize("cut", ["last", "first", "vocabulary", "every_fourth", "one_row", "expanded"])
+def test_gradients_of_sliced_logits(dtype, V, cut):
+    """The gradient's rows start at the logits' offsets from a 16-byte boundary
+    (both are then accessed 16 bytes at a time), in no more memory than its own
+    rows with up to 15 bytes between them take; its values are those of a dense
+    copy."""
+    import mogt_b200
+    g = torch.Generator(device="cuda").manual_seed(3)
+    full = torch.randn(4, 12, V, generator=g, device="cuda").to(dtype)
+    x = {"last": lambda: full[:, :-1], "first": lambda: full[:, 1:], "vocabulary": lambda: full[..., 7:107],
+         "every_fourth": lambda: full[:, ::4], "one_row": lambda: full[:, 5:6],
+         "expanded": lambda: full[:1].expand(4, -1, -1)}[cut]()
+    B, L, n = x.shape
+    lab = torch.randint(0, n, (B, L), generator=g, device="cuda")
+    adv = torch.randn(B, generator=g, device="cuda")
+    old = torch.full((B, L), -7.0, device="cuda")
+
+    def grads(v):
+        v = v.detach().requires_grad_(True)
+        out = [torch.autograd.grad(mogt_b200.policy_loss(v, lab, old, adv), v)[0],
+               torch.autograd.grad(mogt_b200.token_logprobs(v, lab).sum(), v)[0],
+               torch.autograd.grad(mogt_b200.preference_loss(v, lab, adv), v)[0]]
+        return out
+
+    dense = grads(x.contiguous())
+    for a, b in zip(grads(x), dense):
+        # sums over a row go by its alignment: each side is good to TOL32 and one rounding
+        assert max_err(a, b) <= TOL32 + 2 * ROUND[dtype]
+        assert torch.equal(_address(a), _address(x))
+        assert a.untyped_storage().nbytes() <= (B * L * n) * a.element_size() + 16 * (B * L + B + 1)
