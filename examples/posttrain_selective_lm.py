@@ -88,7 +88,7 @@ def main(argv=None):
         # pairs: the better half of the batch against the worse half
         order = torch.argsort(r, descending=True)
         order = order[:2 * (args.batch // 2)]
-        pref = mogt_b200.preference_loss(model(ids[order]), labels[order], ref.sum(1)[order], beta=0.1,
+        pref = mogt_b200.preference_loss(model(ids[order]), labels[order], ref.double().sum(1)[order], beta=0.1,
                                          mask=mask[order])
         opt.zero_grad()
         pref.backward()

@@ -62,6 +62,11 @@ int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, const int64_t* 
  * mogt_logprob_bwd with coef_div = L. */
 int mogt_preference_pairs(const float* logprobs, const float* ref, int64_t P, int64_t L, float beta,
                           float eps, float* loss, float* seq, float* coef, void* stream);
+/* The same with reference sums in f64: at a sum of -30000 one unit of f32 is
+ * 2e-3, far more than the kernel's own f64 sums are off. */
+int mogt_preference_pairs_f64(const float* logprobs, const double* ref, int64_t P, int64_t L,
+                              float beta, float eps, float* loss, float* seq, float* coef,
+                              void* stream);
 
 #ifdef __cplusplus
 }

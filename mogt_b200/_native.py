@@ -90,6 +90,7 @@ SIGNATURES = {
     "mogt_policy_loss": (_int, [_vp, _i64, _i64] + [_vp] * 5 + [_i64, _i64] + [_f32] * 3 + [_vp] * 5
                          + [_i64, _i64] + [_i64] * 3 + [_int, _vp, _sz, _vp]),
     "mogt_preference_pairs": (_int, [_vp, _vp, _i64, _i64, _f32, _f32] + [_vp] * 4),
+    "mogt_preference_pairs_f64": (_int, [_vp, _vp, _i64, _i64, _f32, _f32] + [_vp] * 4),
 }
 
 _lib = None

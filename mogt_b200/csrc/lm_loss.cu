@@ -319,8 +319,10 @@ __device__ __forceinline__ float log_sigmoid(float x) { return fminf(x, 0.f) - l
 
 // One CTA, a warp per pair: the sums of its two sequences and their difference
 // stay in f64 up to the logit (two sums of thousands differ by a few units).
-__global__ void __launch_bounds__(1024) pairs_kernel(const float* lp, const float* ref, int64_t P, int64_t L,
-                                                     float beta, float eps, float* loss, float* seq, float* coef) {
+// R: float or double, the reference sums as they are given.
+template <typename R>
+__global__ void __launch_bounds__(1024) pairs_kernel(const float* lp, const R* ref, int64_t P, int64_t L, float beta,
+                                                     float eps, float* loss, float* seq, float* coef) {
   __shared__ double sm[32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   double tot = 0.0;
@@ -454,10 +456,23 @@ extern "C" int mogt_policy_loss(const void* logits, int64_t sb, int64_t sl, cons
   });
 }
 
-extern "C" int mogt_preference_pairs(const float* logprobs, const float* ref, int64_t P, int64_t L, float beta,
-                                     float eps, float* loss, float* seq, float* coef, void* stream) {
+namespace {
+template <typename R>
+int preference_pairs(const float* logprobs, const R* ref, int64_t P, int64_t L, float beta, float eps, float* loss,
+                     float* seq, float* coef, void* stream) {
   if (P < 0 || L < 0) return MOGT_ERR_SHAPE;
   if (!loss || (P > 0 && (!ref || !seq || !coef || (L > 0 && !logprobs)))) return MOGT_ERR_ARG;
-  pairs_kernel<<<1, 1024, 0, (cudaStream_t)stream>>>(logprobs, ref, P, L, beta, eps, loss, seq, coef);
+  pairs_kernel<R><<<1, 1024, 0, (cudaStream_t)stream>>>(logprobs, ref, P, L, beta, eps, loss, seq, coef);
   return mogt_host::launch_status();
+}
+}  // namespace
+
+extern "C" int mogt_preference_pairs(const float* logprobs, const float* ref, int64_t P, int64_t L, float beta,
+                                     float eps, float* loss, float* seq, float* coef, void* stream) {
+  return preference_pairs(logprobs, ref, P, L, beta, eps, loss, seq, coef, stream);
+}
+
+extern "C" int mogt_preference_pairs_f64(const float* logprobs, const double* ref, int64_t P, int64_t L, float beta,
+                                         float eps, float* loss, float* seq, float* coef, void* stream) {
+  return preference_pairs(logprobs, ref, P, L, beta, eps, loss, seq, coef, stream);
 }

@@ -208,8 +208,8 @@ def _preference(logits, labels, mask, ref, beta, eps, want_grad):
     loss = torch.empty((), dtype=torch.float32, device=dev)
     seq = torch.empty(B, dtype=torch.float32, device=dev)
     coef = torch.empty(B, dtype=torch.float32, device=dev)
-    N.launch("mogt_preference_pairs", dev, lp.data_ptr(), ref.data_ptr(), B // 2, L, beta, eps, loss.data_ptr(),
-             seq.data_ptr(), coef.data_ptr())
+    N.launch("mogt_preference_pairs_f64" if ref.dtype == torch.float64 else "mogt_preference_pairs", dev,
+             lp.data_ptr(), ref.data_ptr(), B // 2, L, beta, eps, loss.data_ptr(), seq.data_ptr(), coef.data_ptr())
     return loss, seq, coef, stats
 
 
@@ -237,7 +237,8 @@ class _PreferenceLossFn(torch.autograd.Function):
 def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0.0, mask=None, return_logprobs=False):
     """Paired preference loss.  Sequences 0..P-1 of the batch are preferred
     over sequences P..2P-1.  With s the sum of a sequence's counting label
-    log-probabilities and ref_logprobs [2P] the reference model's sums,
+    log-probabilities and ref_logprobs [2P] the reference model's sums (float64
+    sums are used as they are, any other type in float32),
 
         x = beta ((s_p - ref_p) - (s_{P+p} - ref_{P+p}))
         loss = mean_p [-(1 - eps) log sigmoid(x) - eps log sigmoid(-x)]
@@ -249,7 +250,10 @@ def preference_loss(logits, labels, ref_logprobs, *, beta=0.1, label_smoothing=0
     logits, labels, mask = _rows(what, logits, labels, mask)
     if logits.shape[0] % 2 or logits.shape[0] == 0:
         raise ValueError(f"{what}: the batch must hold preferred sequences and as many others after them")
-    ref = _token_f32(what, "ref_logprobs", ref_logprobs, labels.shape[:1])
+    if ref_logprobs.dtype == torch.float64 and ref_logprobs.shape == labels.shape[:1]:
+        ref = ref_logprobs.detach().contiguous()
+    else:
+        ref = _token_f32(what, "ref_logprobs", ref_logprobs, labels.shape[:1])
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"{what}: label_smoothing must lie in [0, 1]")
     if torch.is_grad_enabled() and logits.requires_grad:

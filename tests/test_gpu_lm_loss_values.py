@@ -104,3 +104,23 @@ def test_gradients_of_sliced_logits(dtype, V, cut):
         assert max_err(a, b) <= TOL32 + 2 * ROUND[dtype]
         assert torch.equal(_address(a), _address(x))
         assert a.untyped_storage().nbytes() <= (B * L * n) * a.element_size() + 16 * (B * L + B + 1)
+
+
+def test_reference_sums_in_float64():
+    """Sums near -40000, where one unit of 32 bits is 4e-3: given in float64
+    they are used as they are.  The pair's logits are then good to the
+    log-probabilities' own errors (see above)."""
+    import mogt_b200
+    B, L, V, beta = 4, 3000, 50, 0.1
+    t = make(B, L, V, F32, seed=5, mask=False)
+    t["logits"] = t["logits"] - 10 * torch.nn.functional.one_hot(t["labels"], V)
+    x = t["logits"].detach().requires_grad_(True)
+    x64 = t["logits"].double().requires_grad_(True)
+    s = torch.log_softmax(x64.detach(), -1).gather(-1, t["labels"][..., None])[..., 0].sum(-1)
+    ref = s + torch.tensor([3.001, -1.002, 0.5003, 2.0004], dtype=torch.float64, device="cuda")
+    loss = mogt_b200.preference_loss(x, t["labels"], ref, beta=beta)
+    loss64, _ = preference_ref(x64, t["labels"], t["counts"], ref, beta, 0.0)
+    tol = (2 * L) ** 0.5 * 2.0 ** -19 * beta
+    assert abs(float(loss.detach()) - float(loss64.detach())) <= tol
+    g, g64 = torch.autograd.grad(loss, x)[0], torch.autograd.grad(loss64, x64)[0]
+    assert max_err(g, g64) <= tol + TOL32
