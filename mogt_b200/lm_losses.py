@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .selective import _CODE, _DTYPES, _cuda, _f32, _ptr
+from .selective import _CODE, _DTYPES, _cuda, _f32, _ptr, _real
 
 __all__ = ["token_logprobs", "policy_loss", "preference_loss"]
 
@@ -164,6 +164,7 @@ class _PolicyLossFn(torch.autograd.Function):
 def _token_f32(what, name, t, shape):
     if t.shape != shape:
         raise ValueError(f"{what}: {name} must be {list(shape)}")
+    _real(what, **{name: t})
     return _f32(t.detach() if t.requires_grad else t)
 
 
@@ -186,6 +187,7 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
     ref = None if ref_logprobs is None else _token_f32(what, "ref_logprobs", ref_logprobs, shape)
     if advantages.shape not in (shape, shape[:1]):
         raise ValueError(f"{what}: advantages must be [B] or [B, L]")
+    _real(what, advantages=advantages)
     adv = advantages.detach() if advantages.requires_grad else advantages
     adv = adv if adv.dtype == torch.float32 else adv.to(torch.float32)
     if not (clip_low >= 0 and clip_high >= 0):
