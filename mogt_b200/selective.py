@@ -32,6 +32,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -42,12 +43,17 @@ _MAX_STATES = 128
 
 
 def _cuda(what, *ts):
+    """The device of all of ts.  The kernels carry no tangents, so that dual
+    tensors are refused as well (their derivative would come out as none)."""
     index = ts[0].get_device()   # -1 on the CPU
     for t in ts:
         if t is not None and (index < 0 or t.get_device() != index):
             if not t.is_cuda or index < 0:
                 raise ValueError(f"{what} requires CUDA tensors")
             raise ValueError(f"{what}: all tensors must be on one device")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in ts):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
     return ts[0].device
 
 

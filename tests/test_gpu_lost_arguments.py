@@ -42,3 +42,24 @@ def test_real_arguments_of_other_types_are_taken():
     x, lab, f = torch.randn(2, 3, 10, device="cuda"), _z(2, 3, dtype=torch.int64), _z(2, 3)
     assert torch.equal(m.policy_loss(x, lab, f, torch.tensor([1, -1], device="cuda")),
                        m.policy_loss(x, lab, f, torch.tensor([1.0, -1.0], device="cuda")))
+
+
+def test_forward_mode_is_refused():
+    """The kernels carry no tangents: a dual tensor must not come out as if its derivative were zero."""
+    import mogt_b200 as m
+    import torch.autograd.forward_ad as fw
+    x, w, u, A, B = _z(2, 5, 8), _z(8, 4), _z(2, 5, 8), -torch.ones(8, 4, device="cuda"), _z(2, 5, 4)
+    lg, lab, f, p = _z(2, 3, 10), _z(2, 3, dtype=torch.int64), _z(2, 3), _z(2)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))
+        for call in (lambda: m.causal_conv(dual(x), w), lambda: m.causal_conv(x, dual(w)),
+                     lambda: m.causal_conv_step(dual(x[:, 0]), _z(2, 3, 8), w),
+                     lambda: m.selective_scan(u, dual(u), A, B, B), lambda: m.selective_scan(u, u, A, dual(B), B),
+                     lambda: m.selective_scan(u, u, A, B, B, initial_state=dual(_z(2, 8, 4))),
+                     lambda: m.selective_scan_step(_z(2, 8, 4), u[:, 0], u[:, 0], dual(A), B[:, 0], B[:, 0]),
+                     lambda: m.token_logprobs(dual(lg), lab), lambda: m.policy_loss(dual(lg), lab, f, p),
+                     lambda: m.preference_loss(dual(lg), lab, p)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        # tensors without a tangent pass through a dual level
+        assert m.causal_conv(x, w).shape == x.shape and m.token_logprobs(lg, lab).shape == lab.shape
