@@ -17,6 +17,8 @@ results do not vary between runs.  Only the logits receive a gradient.
 """
 from __future__ import annotations
 
+import warnings
+
 import torch
 
 from . import _native as N
@@ -176,8 +178,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
 
     with lp = log softmax(logits)[label], r = exp(lp - old_logprobs),
     d = ref_logprobs - lp and a the advantage.  old_logprobs, ref_logprobs:
-    [B, L] (without ref_logprobs there is no KL term, whatever kl_coef is);
-    advantages: [B] or [B, L].
+    [B, L] (without ref_logprobs there is no KL term, whatever kl_coef is; a
+    weight left unused that way is warned of); advantages: [B] or [B, L].
     Returns the loss (fp32 scalar), with ``return_logprobs`` also lp [B, L]."""
     what = "policy_loss"
     _cuda(what, logits, labels, old_logprobs, advantages, ref_logprobs, mask)
@@ -190,6 +192,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
     _real(what, advantages=advantages)
     adv = advantages.detach() if advantages.requires_grad else advantages
     adv = adv if adv.dtype == torch.float32 else adv.to(torch.float32)
+    if ref_logprobs is None and kl_coef != 0:
+        warnings.warn(f"{what}: kl_coef has no effect without ref_logprobs", stacklevel=2)
     if not (clip_low >= 0 and clip_high >= 0):
         raise ValueError(f"{what}: clip_low and clip_high must not be negative")
     if torch.is_grad_enabled() and logits.requires_grad:

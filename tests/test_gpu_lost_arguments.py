@@ -63,3 +63,17 @@ def test_forward_mode_is_refused():
                 call()
         # tensors without a tangent pass through a dual level
         assert m.causal_conv(x, w).shape == x.shape and m.token_logprobs(lg, lab).shape == lab.shape
+
+
+def test_a_kl_weight_without_reference_is_said():
+    """Without ref_logprobs there is no KL term, whatever its weight; that a weight is left unused is not kept silent."""
+    import warnings
+
+    import mogt_b200 as m
+    x, lab, f, p = _z(2, 3, 10), _z(2, 3, dtype=torch.int64), _z(2, 3), _z(2)
+    with pytest.warns(UserWarning, match="ref_logprobs"):
+        m.policy_loss(x, lab, f, p, kl_coef=0.05)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        m.policy_loss(x, lab, f, p)
+        m.policy_loss(x, lab, f, p, ref_logprobs=f, kl_coef=0.05)
