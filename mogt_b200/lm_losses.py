@@ -22,7 +22,7 @@ import warnings
 import torch
 
 from . import _native as N
-from .selective import _CODE, _DTYPES, _cuda, _f32, _ptr, _real
+from .selective import _CODE, _DTYPES, _cuda, _f32, _ptr
 
 __all__ = ["token_logprobs", "policy_loss", "preference_loss"]
 
@@ -166,7 +166,6 @@ class _PolicyLossFn(torch.autograd.Function):
 def _token_f32(what, name, t, shape):
     if t.shape != shape:
         raise ValueError(f"{what}: {name} must be {list(shape)}")
-    _real(what, **{name: t})
     return _f32(t.detach() if t.requires_grad else t)
 
 
@@ -189,9 +188,8 @@ def policy_loss(logits, labels, old_logprobs, advantages, *, ref_logprobs=None, 
     ref = None if ref_logprobs is None else _token_f32(what, "ref_logprobs", ref_logprobs, shape)
     if advantages.shape not in (shape, shape[:1]):
         raise ValueError(f"{what}: advantages must be [B] or [B, L]")
-    _real(what, advantages=advantages)
     adv = advantages.detach() if advantages.requires_grad else advantages
-    adv = adv if adv.dtype == torch.float32 else adv.to(torch.float32)
+    adv = adv if adv.dtype == torch.float32 else _f32(adv)
     if ref_logprobs is None and kl_coef != 0:
         warnings.warn(f"{what}: kl_coef has no effect without ref_logprobs", stacklevel=2)
     if not (clip_low >= 0 and clip_high >= 0):

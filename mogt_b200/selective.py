@@ -85,16 +85,12 @@ def _lengths(lengths, B, what):
 
 
 def _f32(t):
+    """Dense and in float32; complex values would lose their imaginary part."""
     if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
         return t
+    if t.is_complex():
+        raise ValueError(f"parameters, states and token values must be real, not {t.dtype}")
     return t.to(torch.float32).contiguous()
-
-
-def _real(what, **ts):
-    """Used in float32: an imaginary part would be lost on the way."""
-    for name, t in ts.items():
-        if t is not None and t.is_complex():
-            raise ValueError(f"{what}: {name} must be real")
 
 
 def _writable(what, new_state):
@@ -249,7 +245,6 @@ def _check_scan(what, u, delta, A, Bm, Cm, D, z, delta_bias):
         raise ValueError(f"{what}: u must be bfloat16, float16 or float32")
     if A.ndim != 2 or A.shape[0] != ch:
         raise ValueError(f"{what}: A must be [D, N]")
-    _real(what, A=A, D=D, delta_bias=delta_bias)
     n = A.shape[1]
     if not 1 <= n <= _MAX_STATES:
         raise ValueError(f"{what}: N must be in [1, {_MAX_STATES}]")
@@ -377,7 +372,6 @@ def selective_scan(u, delta, A, B, C, *, D=None, z=None, delta_bias=None, delta_
     Bm, Cm = _check_scan(what, u, delta, A, B, C, D, z, delta_bias)
     if initial_state is not None and initial_state.shape != (u.shape[0], u.shape[2], A.shape[1]):
         raise ValueError(f"{what}: initial_state must be [B, D, N]")
-    _real(what, initial_state=initial_state)
     lengths = _lengths(lengths, u.shape[0], what)
     u, delta, z = _dense_last(u), _dense_last(delta), _dense_last(z)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad
