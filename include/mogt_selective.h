@@ -63,7 +63,8 @@ int mogt_causal_conv_step(const void* x, int64_t x_sb, const void* state, const 
  *   y_t[d]    = sum_n C_t[g, n] h_t[d, n] + Dskip[d] u_t[d]
  *   out_t     = y_t silu(z_t)   (z given)   or   y_t
  * where g = d / (D / G) is the channel's group.
- * Limits: N <= 128, D a multiple of G.
+ * Limits: N <= 128, D a multiple of G, B <= 65535 for the scan; for the single
+ * token D times N / 4, rounded up to a power of two, below 2^31.
  * ------------------------------------------------------------------------- */
 typedef struct mogt_selective_args {
   const void *u, *delta, *z, *Bm, *Cm;            /* z may be NULL */
@@ -89,7 +90,10 @@ typedef struct mogt_selective_args {
 } mogt_selective_args;
 
 /* Bytes of `saved` (the states a backward starts from; f32, one per 16
- * tokens) and of each direction's scratch. */
+ * tokens) and of each direction's scratch.  Most of the backward's holds
+ * partial rows of dB and dC, one per token and block of 256 / (N / 4) channels:
+ * it grows with D N^2 (D = 1536: 3 KB a token at N = 16, 49 KB at 64, 197 KB at
+ * 128). */
 size_t mogt_selective_saved_bytes(int64_t B, int64_t L, int64_t D, int64_t N);
 size_t mogt_selective_fwd_scratch_bytes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G);
 size_t mogt_selective_bwd_scratch_bytes(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G);

@@ -495,7 +495,7 @@ extern "C" int mogt_causal_conv_fwd(const void* x, int64_t x_sb, int64_t x_sl, c
 
 extern "C" size_t mogt_causal_conv_bwd_scratch_bytes(int64_t B, int64_t L, int64_t D, int64_t K) {
   if (B <= 0 || L < 0 || D <= 0) return 0;
-  // the narrowest access has the shortest runs
+  // a row per run: the widest access has the shortest runs, the most rows
   int64_t most = 0;
   for (int v = 1; v <= 4; v <<= 1) {
     const int64_t runs = num_runs(L, run_len(B, L, D, v, kBwdCtas));

@@ -24,9 +24,10 @@
 // are needed.  The CTA's warps add through shared memory and CTAs through a
 // second kernel, in a fixed order.
 //
-// 8192 x 1536 x 16 bf16: 320 us, with the first pass 402.  Bound by
-// shared-memory wavefronts (62 % of their peak) together with instruction
-// issue (54 %); HBM is at 8 %.
+// 8192 x 1536 x 16 bf16: 320 us, with the first pass 402.  Nothing is at its
+// limit: shared-memory wavefronts at 62 % of their peak, instruction issue at
+// 54 % and HBM at 8 %, with 17 % of the warps resident, so that each waits on
+// its own shuffles and shared memory.
 #include "selective_scan.cuh"
 
 namespace mogt {
@@ -35,7 +36,8 @@ namespace sel {
 // CTAs on an SM by registers and shared memory.  For 4 lanes per pair (N = 16)
 // three of 168 registers: 355 us at 8192 x 1536 (320 us since operands are
 // copied asynchronously), against 427 us for two of 255 and 439 us for four of
-// 128, which spill.
+// 128, which spill.  The others (two; one for N <= 4, whose lanes hold most
+// tokens and registers) were not measured against their neighbours.
 constexpr int bwd_ctas(int lpc) { return lpc == 4 ? 3 : lpc == 1 ? 1 : 2; }
 // The first pass over a split sequence costs about a quarter of the main one.
 inline int64_t bwd_segments(int64_t B, int64_t L, int64_t D, int64_t N, int64_t G) {

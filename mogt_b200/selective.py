@@ -361,7 +361,8 @@ def selective_scan(u, delta, A, B, C, *, D=None, z=None, delta_bias=None, delta_
     u, delta, z: [B, L, D]; A: [D, N] (negative for a decaying state); B, C:
     [B, L, N], or [B, L, G, N] when channels form G equal groups; D,
     delta_bias: [D]; initial_state: [B, D, N].  u, delta, z, B and C share one
-    of bfloat16, float16 and float32; the others are used in float32; N <= 128.
+    of bfloat16, float16 and float32; the others are used in float32; N <= 128,
+    at most 65535 sequences.
     Returns y [B, L, D] in u's dtype, with ``return_state`` also the state
     after the last token, [B, D, N] float32, which a later call or
     selective_scan_step takes."""
