@@ -93,7 +93,11 @@ def _f32(t):
     return t.to(torch.float32).contiguous()
 
 
-def _writable(what, new_state):
+def _writable(what, state, new_state):
+    if new_state is not state:
+        apart = abs(new_state.data_ptr() - state.data_ptr())
+        if 0 < apart < state.numel() * state.element_size():
+            raise ValueError(f"{what}: state and new_state overlap")
     if new_state.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{what}: the state to write requires grad, and the call records none: "
                          "detach it, or call under torch.no_grad()")
@@ -201,7 +205,8 @@ def causal_conv(x, weight, bias=None, *, activation="silu", initial_state=None, 
 
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_state=None):
     """One token of causal_conv: x [B, D], state [B, K-1, D] (dense).  Returns
-    y [B, D]; the state shifted by x goes into ``new_state`` (default: state)."""
+    y [B, D]; the state shifted by x goes into ``new_state`` (default: state;
+    another buffer must lie apart from it)."""
     what = "causal_conv_step"
     if x.ndim != 2 or x.dtype not in _DTYPES:
         raise ValueError(f"{what}: x must be [B, D] bfloat16, float16 or float32")
@@ -214,7 +219,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", new_stat
     for s in (state, new_state):
         if s.shape != (B, K - 1, D) or s.dtype != x.dtype or not s.is_contiguous():
             raise ValueError(f"{what}: state must be a contiguous [B, K-1, D] in x's dtype")
-    _writable(what, new_state)
+    _writable(what, state, new_state)
     x = _dense_last(x)
     y = torch.empty(B, D, dtype=x.dtype, device=dev)
     N.launch("mogt_causal_conv_step", dev, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _ptr(bias),
@@ -389,7 +394,8 @@ def selective_scan_step(state, u, delta, A, B, C, *, D=None, z=None, delta_bias=
                         new_state=None):
     """One token of selective_scan: state [B, D, N] float32 (dense), u, delta,
     z [B, D], B and C [B, N] or [B, G, N].  Returns y [B, D] in u's dtype; the
-    state after the token goes into ``new_state`` (default: state)."""
+    state after the token goes into ``new_state`` (default: state; another
+    buffer must lie apart from it)."""
     what = "selective_scan_step"
     if u.ndim != 2:
         raise ValueError(f"{what}: u must be [B, D]")
@@ -401,7 +407,7 @@ def selective_scan_step(state, u, delta, A, B, C, *, D=None, z=None, delta_bias=
     for s in (state, new_state):
         if s.shape != (bs, ch, n) or s.dtype != torch.float32 or not s.is_contiguous():
             raise ValueError(f"{what}: state must be a contiguous [B, D, N] float32")
-    _writable(what, new_state)
+    _writable(what, state, new_state)
     u, delta, z = _dense_last(u), _dense_last(delta), _dense_last(z)
     A, D, delta_bias = _f32(A), _f32(D), _f32(delta_bias)
     y = torch.empty(bs, ch, dtype=u.dtype, device=dev)

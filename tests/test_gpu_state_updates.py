@@ -78,3 +78,20 @@ def test_steps_in_inference_mode():
         assert torch.equal(st[:, :-1], before[:, 1:]) and torch.equal(st[:, -1], x[:, 0])
         u, delta, A, B, C, st = _scan()
         mogt_b200.selective_scan_step(st, u[:, 0], delta[:, 0], A, B[:, 0], C[:, 0])
+
+
+def test_overlapping_states_are_refused():
+    """A new state may be the old one or lie apart from it: threads of one sequence would write what others still read."""
+    import mogt_b200
+    x, w, _ = _conv()
+    buf = torch.randn(3, 3, 8, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        mogt_b200.causal_conv_step(x[:, 0], buf[:2], w, new_state=buf[1:])
+    mogt_b200.causal_conv_step(x[:, 0], buf[:2], w, new_state=buf[:2])
+    u, delta, A, B, C, _ = _scan()
+    buf = torch.randn(4, 8, 4, device="cuda")
+    step = [u[:, 0], delta[:, 0], A, B[:, 0], C[:, 0]]
+    for state, new in ((buf[:2], buf[1:3]), (buf[1:3], buf[:2])):
+        with pytest.raises(ValueError, match="overlap"):
+            mogt_b200.selective_scan_step(state, *step, new_state=new)
+    mogt_b200.selective_scan_step(buf[:2], *step, new_state=buf[2:])
